@@ -274,7 +274,7 @@ def _run_own(s):
                                      group_top=s["group_top"], **kind)
         if p == "route":
             return ids, weights
-        return ids, weights, ops.moe_route_backward(s["grad"], s["logits"], ids, **kind)
+        return ids, weights, ops.moe_route_backward(s["grad"], s["logits"], ids, weights, **kind)
     if p == "quant":
         q, sf = ops.quantize_fp8_block(s["x"], silu=s["silu"], group_offsets=s.get("offsets"), group_rows=s.get("group_rows"),
                                        out=(s["q"], s["sf"]))
