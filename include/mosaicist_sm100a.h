@@ -285,6 +285,40 @@ int msc_grouped_gemm_bf16_int4_ragged(const void* a, const void* b_q, const void
                                       const int32_t* group_rows, void* out, int l, int rows_total,
                                       int n, int k, int group_size, int max_ctas, void* stream);
 
+/* ---- FP8 with fp32 scales per block of 128 ---------------------------------------------
+ * e4m3 values, activations with one scale per row and 128 columns, weights with one per 128 x 128
+ * block (the structure of the reference's block-scaled FP8 quantiser,
+ * experiments/flashinfer-megamoe-sm90a/quant.py:47-75):
+ *   scale = max(amax / 448, 2^-126), q = e4m3_rne(fp32(x / scale)).
+ * Types: 0 bf16, 1 f32, 2 f16.  k % 16 == 0 throughout; a last block of fewer than 128 columns or rows
+ * is a block of its own. */
+
+/* x (rows, k), or with silu (rows, 2k) gate | up of which silu(gate) * up is taken in fp32 -> q (rows, k)
+ * bytes, sf (ceil(k / 128), pitch) f32 with pitch = rows rounded up to 4; the columns behind `rows`
+ * become 0.  With group_offsets / group_rows (l) only rows inside a group are read and written; groups
+ * may start anywhere.  rows <= 524280; rows = 0 does nothing. */
+int msc_fp8_block_quantize(const void* x, int x_dtype, int silu, const int32_t* group_offsets,
+                           const int32_t* group_rows, void* q, float* sf, int l, int rows, int k, void* stream);
+
+/* w (l, n, k) -> q (l, n, k) bytes, sf (l, ceil(n / 128), ceil(k / 128)) f32. */
+int msc_fp8_block_quantize_weight(const void* w, int w_dtype, void* q, float* sf, int l, int n, int k,
+                                  void* stream);
+
+/* out (m, n) = dequant(a) (m, k) x dequant(b) (n, k)^T, fp32 sums, out_dtype as above.  a_sf as
+ * msc_fp8_block_quantize lays it out (pitch = m rounded up to 4), b_sf (ceil(n / 128), ceil(k / 128)).
+ * n % 8 == 0.  max_ctas: CTAs of the launch, 0 = all SMs.  m = 0 does nothing. */
+int msc_gemm_fp8_block(const void* a_q, const float* a_sf, const void* b_q, const float* b_sf, void* out,
+                       int out_dtype, int m, int n, int k, int max_ctas, void* stream);
+
+/* The same for each group of a row-concatenated batch: group g owns rows [group_offsets[g], +
+ * group_rows[g]) of a_q (rows_total, k) and out (rows_total, n) and the weights b_q[g] (n, k).  Groups may
+ * start anywhere; what reaches beyond rows_total is cut off; rows outside the groups are left as they
+ * are.  row_scale (rows_total) f32 or NULL multiplies the rows before they are rounded. */
+int msc_grouped_gemm_fp8_block_ragged(const void* a_q, const float* a_sf, const void* b_q, const float* b_sf,
+                                      const int32_t* group_offsets, const int32_t* group_rows,
+                                      const float* row_scale, void* out, int out_dtype, int l, int rows_total,
+                                      int n, int k, int max_ctas, void* stream);
+
 /* ---- MoE routing and token movement ---------------------------------------------------
  * The reference's MoE takes per-expert padded batches and has no routing, permutation or
  * exchange code (experiments/flashinfer-megamoe-sm100a/moe.py:47-79; the only hint is that
@@ -297,6 +331,37 @@ int msc_grouped_gemm_bf16_int4_ragged(const void* a, const void* b_q, const void
  * logits (tokens, experts) f32 -> ids (tokens, topk) i32, weights (tokens, topk) f32. */
 int msc_moe_route_topk(const float* logits, int32_t* ids, float* weights, int tokens, int experts,
                        int topk, void* stream);
+
+#define MSC_SCORE_SOFTMAX 0
+#define MSC_SCORE_SIGMOID 1
+
+/* How msc_moe_route scores and chooses. */
+typedef struct msc_route_cfg {
+  int score;         /* MSC_SCORE_SOFTMAX over all experts, or MSC_SCORE_SIGMOID of each logit          */
+  int groups;        /* experts form this many equal groups of neighbours (1: no groups), <= 32         */
+  int topk_groups;   /* the best so many groups take part                                               */
+  int group_top;     /* a group's key is the sum of its best 1 or 2 keys                                */
+  int renormalize;   /* weights are divided by the sum of the chosen scores                             */
+  float scale;       /* and multiplied by this, > 0                                                     */
+} msc_route_cfg;
+
+/* Routing with the choices of current mixtures of experts: key = score + bias (bias (experts) f32 or
+ * NULL; it takes part in the choice, not in the weights), the best topk_groups groups, of their
+ * experts the `topk` best keys in falling order, weights from the chosen scores.  Ties go to the lower
+ * group and expert; the order is that of 64-bit arithmetic.  A logit or bias that is -inf or NaN bars
+ * its expert; where fewer than topk are left the lowest barred ones fill up, with weight 0.
+ * logits (tokens, experts), dtype 0 bf16, 1 f32, 2 f16 -> ids (tokens, topk) i32, weights (tokens, topk) f32.
+ * experts <= 1024, groups * ceil(experts / groups / 32) <= 32, topk <= 32 and at most the experts of
+ * topk_groups groups.  tokens = 0 does nothing. */
+int msc_moe_route(const void* logits, int dtype, const float* bias, int32_t* ids, float* weights, int tokens,
+                  int experts, int topk, const msc_route_cfg* cfg, void* stream);
+
+/* Gradient of the logits (tokens, experts; type of the logits) from the gradient of the weights and
+ * what msc_moe_route returned for them.  The choice itself has no gradient, and so neither have the
+ * bias and the experts that were not chosen, but for the sum in a softmax that is not renormalised. */
+int msc_moe_route_backward(const float* grad_weights, const void* logits, int dtype, const int32_t* ids,
+                           const float* weights, void* grad_logits, int tokens, int experts, int topk, int score,
+                           int renormalize, float scale, void* stream);
 
 /* For the experts [expert_first, expert_first + experts_local): rows per expert, the rank of
  * every (token, k) pair inside its expert (token order), and 128-aligned group offsets.

@@ -16,6 +16,7 @@ LIB_PATH = pathlib.Path(os.environ.get("MSC_LIB_PATH") or PKG / "libmosaicist_sm
 
 OK, ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_SMEM, ERR_CUDA, ERR_TIMEOUT = 0, -1, -2, -3, -4, -5
 EPI_PLAIN, EPI_ROW_SCALE = 0, 1
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 
 
 class MscError(RuntimeError):
@@ -28,6 +29,11 @@ class GemmCfg(ctypes.Structure):
     _fields_ = [("tile_n", ctypes.c_int), ("stages", ctypes.c_int), ("raster", ctypes.c_int),
                 ("max_ctas", ctypes.c_int), ("epilogue", ctypes.c_int),
                 ("cta_pair", ctypes.c_int), ("sf_warps", ctypes.c_int), ("reserved", ctypes.c_int)]
+
+
+class RouteCfg(ctypes.Structure):
+    _fields_ = [("score", ctypes.c_int), ("groups", ctypes.c_int), ("topk_groups", ctypes.c_int),
+                ("group_top", ctypes.c_int), ("renormalize", ctypes.c_int), ("scale", ctypes.c_float)]
 
 
 _P, _I = ctypes.c_void_p, ctypes.c_int
@@ -62,6 +68,12 @@ SIGNATURES = {
     "msc_grouped_gemm_bf16_int4_ragged": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
     "msc_swiglu_interleave_w1": (_I, [_P, _P, _P, _P, _I, _I, _I, _P]),
     "msc_moe_route_topk": (_I, [_P, _P, _P, _I, _I, _I, _P]),
+    "msc_moe_route": (_I, [_P, _I, _P, _P, _P, _I, _I, _I, ctypes.POINTER(RouteCfg), _P]),
+    "msc_moe_route_backward": (_I, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_float, _P]),
+    "msc_fp8_block_quantize": (_I, [_P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "msc_fp8_block_quantize_weight": (_I, [_P, _I, _P, _P, _I, _I, _I, _P]),
+    "msc_gemm_fp8_block": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
+    "msc_grouped_gemm_fp8_block_ragged": (_I, [_P] * 8 + [_I] * 6 + [_P]),
     "msc_moe_plan": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
     "msc_moe_plan_noalloc": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P]),
     "msc_moe_permute_quantize": (_I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P]),

@@ -1,0 +1,274 @@
+// FP8 with one fp32 scale per block: activations in blocks of 1 x 128, weights of 128 x 128 (both HBM-bound).
+//
+//   s = max(amax / 448, 2^-126)     in fp32, amax the block's largest magnitude, NaNs left out
+//   q = e4m3_rne(x / s)             the quotient rounded to fp32 first
+// (structure of the reference's block-scaled FP8 quantiser, experiments/flashinfer-megamoe-sm90a/quant.py:47-75,
+// with fp32 scales per 128).  The floor of the scale keeps x / s finite in a block of zeros.  An
+// infinite element makes its block's scale infinite: infinities come out NaN, the others 0.  NaN stays NaN.
+//
+// The scales of activations are laid out by block column, (ceil(k / 128), rows rounded up to 4): what the
+// product reads for a tile of rows and one K step is then one contiguous, 16-byte aligned piece.
+#include "host_common.h"
+#include "ptx.cuh"
+#include "quantize_common.cuh"
+
+#include <cuda_fp16.h>
+
+namespace msc {
+
+constexpr float kFp8Max = 448.0f;
+constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126
+
+__device__ __forceinline__ float block_scale(float amax) { return fmaxf(__fdiv_rn(amax, kFp8Max), kLeastScale); }
+
+// 16 values / s -> 16 bytes of e4m3.  The quotients are those of __fdiv_rn wherever they decide an e4m3
+// value, at three instructions for two of them (div_rn_shared_rcp; the remainder is exact while s is well inside
+// fp32's exponents, and quotients below 2^-10 round to zero whatever their last bit is).
+__device__ __forceinline__ uint4 pack_e4m3_16(const float* v, float s) {
+  const bool mid = s >= 1e-25f && s <= 1e25f;
+  const float r = __frcp_rn(s);
+  const uint64_t r2 = pair_f32(r, r), n2 = pair_f32(-s, -s);
+  uint32_t w[4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    float2 x[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float a = v[4 * h + 2 * j], b = v[4 * h + 2 * j + 1];
+      if (mid) {
+        const uint64_t a2 = pair_f32(a, b);
+        const uint64_t q2 = mul_f32x2(a2, r2);
+        x[j] = unpair_f32(fma_f32x2(fma_f32x2(q2, n2, a2), r2, q2));
+      } else {
+        x[j] = make_float2(__fdiv_rn(a, s), __fdiv_rn(b, s));
+      }
+    }
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(x[0], __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(x[1], __NV_SATFINITE, __NV_E4M3);
+    w[h] = lo | (hi << 16);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Eight 16-bit or four 32-bit values of a 16-byte vector as fp32.
+template <class T> struct Vec16;
+template <> struct Vec16<__nv_bfloat16> {
+  static constexpr int kPer = 8;
+  static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+};
+template <> struct Vec16<__half> {
+  static constexpr int kPer = 8;
+  static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+};
+template <> struct Vec16<float> {
+  static constexpr int kPer = 4;
+  static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+    v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y);
+    v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+  }
+};
+
+// 16 consecutive values (16-byte aligned).
+template <class T>
+__device__ __forceinline__ void load_16(const T* src, float* v) {
+  constexpr int kVecs = 16 / Vec16<T>::kPer;
+  uint4 raw[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) raw[i] = ld_ordered(reinterpret_cast<const uint4*>(src) + i);
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) Vec16<T>::unpack(raw[i], v + i * Vec16<T>::kPer);
+}
+
+struct RowBlockParams {
+  const void* x;             // (rows, k), with SILU (rows, 2k) gate | up
+  uint8_t* q;                // (rows, k)
+  float* sf;                 // (kblocks, pitch)
+  const int* group_offsets;  // [l] or null: every row
+  const int* group_rows;     // [l]
+  int l, rows, pitch, k, kblocks;
+};
+
+// ---- activations ---------------------------------------------------------------------------
+// A CTA takes 8 rows x 512 columns, a warp one of the rows, a thread 16 values: 8 lanes share a block.  The
+// 32 scales of the tile meet in shared memory and leave as 32-byte pieces of the column layout.
+template <class T, bool SILU>
+__global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const RowBlockParams p) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  __shared__ float s_scale[8][4];
+  __shared__ unsigned s_live;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row0 = blockIdx.y * 8, row = row0 + warp;
+  const int col = blockIdx.x * 512 + lane * 16;
+
+  // the rows of the tile that take part: all of them, or those that some group owns
+  unsigned live = row0 + 8 <= p.rows ? 0xffu : (1u << max(p.rows - row0, 0)) - 1u;
+  if (p.group_offsets) {
+    if (threadIdx.x == 0) s_live = 0u;
+    __syncthreads();
+    for (int g = threadIdx.x; g < p.l; g += 256) {
+      const long long off = ld_ordered(p.group_offsets + g);
+      const long long lo = max(off - row0, 0LL), hi = min(off + ld_ordered(p.group_rows + g) - row0, 8LL);
+      if (off >= 0 && lo < hi) atomicOr(&s_live, ((1u << (int)hi) - 1u) & ~((1u << (int)lo) - 1u));
+    }
+    __syncthreads();
+    live &= s_live;
+  }
+  if (live || row0 + 8 > p.rows) {   // (the last rows' tile also clears the scale columns behind them)
+    const bool mine = ((live >> warp) & 1u) && col < p.k;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    if (mine) {
+      if (SILU) {
+        const T* src = static_cast<const T*>(p.x) + (size_t)row * 2 * p.k + col;
+        float up[16];
+        load_16(src, v);
+        load_16(src + p.k, up);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = silu_mul(v[i], up[i]);
+      } else {
+        load_16(static_cast<const T*>(p.x) + (size_t)row * p.k + col, v);
+      }
+    }
+    float amax = amax_f32x16(v);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float s = block_scale(amax);
+    if ((lane & 7) == 0) s_scale[warp][lane >> 3] = s;
+    if (mine) *reinterpret_cast<uint4*>(p.q + (size_t)row * p.k + col) = pack_e4m3_16(v, s);
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const int c = blockIdx.x * 4 + (threadIdx.x >> 3), r = threadIdx.x & 7;
+      if (c < p.kblocks) {
+        if ((live >> r) & 1u) p.sf[(size_t)c * p.pitch + row0 + r] = s_scale[r][threadIdx.x >> 3];
+        else if (row0 + r >= p.rows && row0 + r < p.pitch) p.sf[(size_t)c * p.pitch + row0 + r] = 0.0f;
+      }
+    }
+  }
+}
+
+// ---- weights -------------------------------------------------------------------------------
+// A CTA per 128 x 128 block, whose values stay in registers between the maximum and the quotients: a
+// thread holds 64 of them in four row pieces of 16.
+struct WeightBlockParams {
+  const void* w;    // (l, n, k)
+  uint8_t* q;       // (l, n, k)
+  float* sf;        // (l, nblocks, kblocks)
+  int n, k, nblocks, kblocks;
+};
+
+template <class T>
+__global__ void __launch_bounds__(256) quantize_fp8_weight_kernel(const WeightBlockParams p) {
+  __shared__ float s_amax[8];
+  constexpr int kVecs = 16 / Vec16<T>::kPer;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const size_t g = blockIdx.z;
+  const int col = blockIdx.x * 128 + (lane & 7) * 16;
+  const int row0 = blockIdx.y * 128 + warp * 4 + (lane >> 3);   // then every 32 rows
+  const T* src = static_cast<const T*>(p.w) + (g * p.n + row0) * p.k + col;
+  uint4 raw[4][kVecs];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j)
+      raw[i][j] = (row0 + 32 * i < p.n && col < p.k) ? __ldg(reinterpret_cast<const uint4*>(src + (size_t)32 * i * p.k) + j)
+                                                     : make_uint4(0u, 0u, 0u, 0u);
+  float amax = 0.0f;
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) Vec16<T>::unpack(raw[i][j], v + j * Vec16<T>::kPer);
+    amax = fmaxf(amax, amax_f32x16(v));
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if (lane == 0) s_amax[warp] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, s_amax[i]);
+  const float s = block_scale(amax);
+  uint8_t* dst = p.q + (g * p.n + row0) * p.k + col;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) Vec16<T>::unpack(raw[i][j], v + j * Vec16<T>::kPer);
+    if (row0 + 32 * i < p.n && col < p.k) *reinterpret_cast<uint4*>(dst + (size_t)32 * i * p.k) = pack_e4m3_16(v, s);
+  }
+  if (threadIdx.x == 0) p.sf[(g * p.nblocks + blockIdx.y) * p.kblocks + blockIdx.x] = s;
+}
+
+template <class T>
+static int launch_rows(const RowBlockParams& p, bool silu, cudaStream_t stream) {
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t lc = pdl_launch_config((p.k + 511) / 512, 256, 0, stream, attr);
+  lc.gridDim.y = (unsigned)((p.rows + 7) / 8);
+  auto kern = silu ? quantize_fp8_rows_kernel<T, true> : quantize_fp8_rows_kernel<T, false>;
+  MSC_CUDA_OK(cudaLaunchKernelEx(&lc, kern, p));
+  return MSC_OK;
+}
+
+}  // namespace msc
+
+extern "C" {
+
+int msc_fp8_block_quantize(const void* x, int x_dtype, int silu, const int32_t* group_offsets, const int32_t* group_rows,
+                           void* q, float* sf, int l, int rows, int k, void* stream) {
+  using namespace msc;
+  if (!x || !q || !sf) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
+  if (!group_offsets != !group_rows) return fail(MSC_ERR_BAD_ARG, "group_offsets and group_rows come together");
+  if (group_offsets && l <= 0) return fail(MSC_ERR_BAD_ARG, "l=%d must be positive with groups", l);
+  if (rows < 0 || k <= 0) return fail(MSC_ERR_BAD_ARG, "rows=%d must not be negative, k=%d must be positive", rows, k);
+  if (k % 16) return fail(MSC_ERR_BAD_ARG, "k=%d must be a multiple of 16", k);
+  if (x_dtype < 0 || x_dtype > 2) return fail(MSC_ERR_UNSUPPORTED, "x_dtype must be 0 (bf16), 1 (f32) or 2 (f16), got %d", x_dtype);
+  if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(sf) % 4)
+    return fail(MSC_ERR_BAD_ARG, "x and q must be 16-byte aligned, sf 4-byte aligned");
+  if (rows > 65535 * 8) return fail(MSC_ERR_UNSUPPORTED, "rows=%d exceeds %d", rows, 65535 * 8);
+  if (rows == 0) return MSC_OK;
+  RowBlockParams p;
+  p.x = x; p.q = static_cast<uint8_t*>(q); p.sf = sf;
+  p.group_offsets = group_offsets; p.group_rows = group_rows; p.l = l;
+  p.rows = rows; p.pitch = (rows + 3) & ~3; p.k = k; p.kblocks = (k + 127) / 128;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return x_dtype == 0 ? launch_rows<__nv_bfloat16>(p, silu != 0, st)
+         : x_dtype == 1 ? launch_rows<float>(p, silu != 0, st) : launch_rows<__half>(p, silu != 0, st);
+}
+
+int msc_fp8_block_quantize_weight(const void* w, int w_dtype, void* q, float* sf, int l, int n, int k, void* stream) {
+  using namespace msc;
+  if (!w || !q || !sf) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
+  if (l <= 0 || n <= 0 || k <= 0) return fail(MSC_ERR_BAD_ARG, "sizes must be positive");
+  if (k % 16) return fail(MSC_ERR_BAD_ARG, "k=%d must be a multiple of 16", k);
+  if (w_dtype < 0 || w_dtype > 2) return fail(MSC_ERR_UNSUPPORTED, "w_dtype must be 0 (bf16), 1 (f32) or 2 (f16), got %d", w_dtype);
+  if (reinterpret_cast<uintptr_t>(w) % 16 || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(sf) % 4)
+    return fail(MSC_ERR_BAD_ARG, "w and q must be 16-byte aligned, sf 4-byte aligned");
+  WeightBlockParams p;
+  p.w = w; p.q = static_cast<uint8_t*>(q); p.sf = sf;
+  p.n = n; p.k = k; p.nblocks = (n + 127) / 128; p.kblocks = (k + 127) / 128;
+  if (l > 65535 || p.nblocks > 65535) return fail(MSC_ERR_UNSUPPORTED, "l=%d or n=%d is too large for one launch", l, n);
+  const dim3 grid((unsigned)p.kblocks, (unsigned)p.nblocks, (unsigned)l);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (w_dtype == 0) quantize_fp8_weight_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p);
+  else if (w_dtype == 1) quantize_fp8_weight_kernel<float><<<grid, 256, 0, st>>>(p);
+  else quantize_fp8_weight_kernel<__half><<<grid, 256, 0, st>>>(p);
+  MSC_CUDA_OK(cudaGetLastError());
+  return MSC_OK;
+}
+
+}  // extern "C"

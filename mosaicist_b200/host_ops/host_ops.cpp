@@ -17,6 +17,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
@@ -47,7 +48,9 @@ using OptTensor = std::optional<Tensor>;
   X(msc_amax_global_scale) X(msc_gemm_f16) X(msc_int4_dequant_bf16)                              \
   X(msc_grouped_gemm_bf16_ragged) X(msc_grouped_gemm_bf16_int4_ragged) X(msc_moe_route_topk)     \
   X(msc_moe_plan) X(msc_moe_permute_quantize) X(msc_moe_unpermute)                               \
-  X(msc_moe_masked_workspace) X(msc_moe_masked)
+  X(msc_moe_masked_workspace) X(msc_moe_masked) X(msc_moe_route) X(msc_moe_route_backward)       \
+  X(msc_fp8_block_quantize) X(msc_fp8_block_quantize_weight) X(msc_gemm_fp8_block)               \
+  X(msc_grouped_gemm_fp8_block_ragged)
 
 struct Lib {
 #define X(name) decltype(&::name) name = nullptr;
@@ -152,7 +155,7 @@ void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
 // ---- argument checks ---------------------------------------------------------------------------
 
-enum Types { kBytes, kF32, kI32, kBf16, kBf16F32, kU8, kPackedInt };
+enum Types { kBytes, kF32, kI32, kBf16, kBf16F32, kU8, kPackedInt, kFloats, kE4m3 };
 
 bool type_ok(at::ScalarType t, Types want) {
   switch (want) {
@@ -165,6 +168,8 @@ bool type_ok(at::ScalarType t, Types want) {
     case kBf16F32: return t == at::kBFloat16 || t == at::kFloat;
     case kU8: return t == at::kByte;
     case kPackedInt: return t == at::kByte || t == at::kChar;
+    case kFloats: return t == at::kBFloat16 || t == at::kFloat || t == at::kHalf;
+    case kE4m3: return t == at::kByte || t == at::ScalarType::Float8_e4m3fn;
   }
   return false;
 }
@@ -177,6 +182,8 @@ const char* type_names(Types want) {
     case kBf16F32: return "bfloat16 or float32";
     case kU8: return "uint8";
     case kPackedInt: return "uint8 or int8";
+    case kFloats: return "bfloat16, float16 or float32";
+    case kE4m3: return "uint8 or float8_e4m3fn";
   }
   return "";
 }
@@ -219,6 +226,27 @@ Tensor empty(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
 }
 
 int dt(const Tensor& x) { return x.scalar_type() == at::kBFloat16 ? 0 : 1; }
+// The same with fp16, for the operators that take all three.
+int dt3(const Tensor& x) { return x.scalar_type() == at::kHalf ? 2 : dt(x); }
+constexpr at::ScalarType kOutTypes[] = {at::kBFloat16, at::kFloat, at::kHalf};
+
+// Every tensor of a call on the device of the first; the launch then runs there, on that device's
+// current stream, whatever device is current.
+void one_device(const Tensor& first, std::initializer_list<std::pair<const Tensor*, const char*>> rest) {
+  for (const auto& [t, name] : rest)
+    if (C10_UNLIKELY(t && t->device() != first.device()))
+      value_error(std::string(name) + " is on " + t->device().str() + ", expected " + first.device().str());
+}
+const Tensor* opt_ptr(const OptTensor& t) { return t ? &*t : nullptr; }
+struct OnDeviceOf {
+  c10::cuda::CUDAGuard guard;
+  void* stream;
+  explicit OnDeviceOf(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+};
+int as_int(int64_t v, const char* name) {
+  if (C10_UNLIKELY(v < 0 || v > 0x7fffffff)) value_error(std::string(name) + "=" + std::to_string(v) + " is out of range");
+  return (int)v;
+}
 
 // ---- the operators on tensors ------------------------------------------------------------------
 
@@ -488,6 +516,179 @@ Tensor gemm_int4_ragged(const Tensor& a, const Tensor& b_q, const Tensor& scales
   return *out;
 }
 
+// ---- routing ------------------------------------------------------------------------------------
+
+std::tuple<Tensor, Tensor> moe_route(const Tensor& logits, int64_t topk, const OptTensor& bias, const msc_route_cfg& cfg,
+                                     OptTensor ids, OptTensor weights) {
+  need(logits, "logits", kFloats);
+  need_dim(logits, "logits", 2);
+  const int64_t tokens = logits.size(0), experts = logits.size(1);
+  if (topk < 1 || topk > experts) value_error("topk=" + std::to_string(topk) + " must be in [1, experts=" + std::to_string(experts) + "]");
+  if (bias) need(*bias, "bias", kF32, {experts});
+  if (ids) {
+    need(*ids, "ids", kI32, {tokens, topk});
+    need(*weights, "weights", kF32, {tokens, topk});
+  }
+  one_device(logits, {{opt_ptr(bias), "bias"}, {opt_ptr(ids), "ids"}, {opt_ptr(weights), "weights"}});
+  const int t = as_int(tokens, "tokens"), e = as_int(experts, "experts");
+  if (!ids) {
+    ids = empty({tokens, topk}, at::kInt, logits);
+    weights = empty({tokens, topk}, at::kFloat, logits);
+  }
+  if (!tokens) return {*ids, *weights};
+  const Lib& f = lib();
+  const OnDeviceOf on(logits);
+  launch([&] {
+    return f.msc_moe_route(ptr(logits), dt3(logits), ptr<float>(bias), static_cast<int32_t*>(ids->data_ptr()),
+                           static_cast<float*>(weights->data_ptr()), t, e, (int)topk, &cfg, on.stream);
+  });
+  return {*ids, *weights};
+}
+
+Tensor moe_route_backward(const Tensor& grad, const Tensor& logits, const Tensor& ids, const Tensor& weights, int score,
+                          bool renormalize, double scale, OptTensor out) {
+  need(logits, "logits", kFloats);
+  need_dim(logits, "logits", 2);
+  need(ids, "ids", kI32);
+  need_dim(ids, "ids", 2);
+  const int64_t tokens = logits.size(0), experts = logits.size(1), topk = ids.size(1);
+  need(ids, "ids", kI32, {tokens, topk});
+  need(weights, "weights", kF32, {tokens, topk});
+  need(grad, "grad_weights", kF32, {tokens, topk});
+  if (out) {
+    need(*out, "out", kFloats, {tokens, experts});
+    if (out->scalar_type() != logits.scalar_type()) value_error("out must have the type of the logits");
+  }
+  one_device(logits, {{&ids, "ids"}, {&weights, "weights"}, {&grad, "grad_weights"}, {opt_ptr(out), "out"}});
+  const int t = as_int(tokens, "tokens"), e = as_int(experts, "experts"), k = as_int(topk, "topk");
+  if (!out) out = empty({tokens, experts}, logits.scalar_type(), logits);
+  if (!tokens) return *out;
+  const Lib& f = lib();
+  const OnDeviceOf on(logits);
+  launch([&] {
+    return f.msc_moe_route_backward(ptr<float>(grad), ptr(logits), dt3(logits), ptr<int32_t>(ids), ptr<float>(weights),
+                                    out->data_ptr(), t, e, k, score, renormalize ? 1 : 0, (float)scale, on.stream);
+  });
+  return *out;
+}
+
+// ---- FP8 with fp32 scales per block of 128 ---------------------------------------------------------
+
+int64_t blocks_of(int64_t v) { return (v + 127) / 128; }
+int64_t pitch_of(int64_t rows) { return (rows + 3) / 4 * 4; }
+
+// clear: rows that no group owns come back as zeros in fresh results.
+std::tuple<Tensor, Tensor> quantize_fp8_block(const Tensor& x, bool silu, const OptTensor& offsets, const OptTensor& rows,
+                                              OptTensor q, OptTensor sf, bool clear) {
+  need(x, "x", kFloats);
+  need_dim(x, "x", 2);
+  const int64_t total = x.size(0), k = silu ? x.size(1) / 2 : x.size(1);
+  if (silu && x.size(1) % 2) value_error("x must have an even number of columns, gate | up, got " + std::to_string(x.size(1)));
+  if (k < 1) value_error("x must have columns");
+  int64_t l = 0;
+  if (offsets.has_value() != rows.has_value()) value_error("group_offsets and group_rows come together");
+  if (offsets) {
+    need_dim(*offsets, "group_offsets", 1);
+    l = offsets->size(0);
+    if (l < 1) value_error("group_offsets must have at least one group");
+    need(*offsets, "group_offsets", kI32, {l});
+    need(*rows, "group_rows", kI32, {l});
+  }
+  if (q) {
+    need(*q, "q", kE4m3, {total, k});
+    need(*sf, "sf", kF32, {blocks_of(k), pitch_of(total)});
+  }
+  one_device(x, {{opt_ptr(offsets), "group_offsets"}, {opt_ptr(rows), "group_rows"}, {opt_ptr(q), "q"}, {opt_ptr(sf), "sf"}});
+  const int n_rows = as_int(total, "rows"), kk = as_int(k, "k"), ll = as_int(l, "l");
+  if (!q) {
+    q = empty({total, k}, at::kByte, x);
+    sf = empty({blocks_of(k), pitch_of(total)}, at::kFloat, x);
+    if (clear && offsets) {
+      q->zero_();
+      sf->zero_();
+    }
+  }
+  if (!total) return {*q, *sf};
+  const Lib& f = lib();
+  const OnDeviceOf on(x);
+  launch([&] {
+    return f.msc_fp8_block_quantize(ptr(x), dt3(x), silu ? 1 : 0, ptr<int32_t>(offsets), ptr<int32_t>(rows), q->data_ptr(),
+                                    static_cast<float*>(sf->data_ptr()), ll, n_rows, kk, on.stream);
+  });
+  return {*q, *sf};
+}
+
+std::tuple<Tensor, Tensor> quantize_fp8_block_weight(const Tensor& w, OptTensor q, OptTensor sf) {
+  need(w, "w", kFloats);
+  if (w.dim() != 2 && w.dim() != 3) value_error("w must be (n, k) or (l, n, k), got shape " + shape_text(w.sizes()));
+  const bool grouped = w.dim() == 3;
+  const int64_t l = grouped ? w.size(0) : 1, n = w.size(-2), k = w.size(-1);
+  const std::vector<int64_t> sizes = grouped ? std::vector<int64_t>{l, blocks_of(n), blocks_of(k)}
+                                             : std::vector<int64_t>{blocks_of(n), blocks_of(k)};
+  if (q) {
+    need(*q, "q", kE4m3);
+    need(*sf, "sf", kF32);
+    if (q->sizes() != w.sizes()) value_error("q has shape " + shape_text(q->sizes()) + ", expected " + shape_text(w.sizes()));
+    if (sf->sizes() != at::IntArrayRef(sizes)) value_error("sf has shape " + shape_text(sf->sizes()) + ", expected " + shape_text(sizes));
+  }
+  one_device(w, {{opt_ptr(q), "q"}, {opt_ptr(sf), "sf"}});
+  const int ll = as_int(l, "l"), nn = as_int(n, "n"), kk = as_int(k, "k");
+  if (!q) {
+    q = empty(w.sizes(), at::kByte, w);
+    sf = empty(sizes, at::kFloat, w);
+  }
+  const Lib& f = lib();
+  const OnDeviceOf on(w);
+  launch([&] {
+    return f.msc_fp8_block_quantize_weight(ptr(w), dt3(w), q->data_ptr(), static_cast<float*>(sf->data_ptr()), ll, nn, kk, on.stream);
+  });
+  return {*q, *sf};
+}
+
+// Dense without offsets: b (n, k); else b (l, n, k).  out_type: index into kOutTypes, or -1 for bf16 or that of `out`.
+Tensor gemm_fp8_block(const Tensor& a_q, const Tensor& a_sf, const Tensor& b_q, const Tensor& b_sf, const OptTensor& offsets,
+                      const OptTensor& rows, const OptTensor& row_scale, int out_type, OptTensor out, int64_t max_ctas) {
+  need(a_q, "a_q", kE4m3);
+  need_dim(a_q, "a_q", 2);
+  need(b_q, "b_q", kE4m3);
+  need_dim(b_q, "b_q", offsets ? 3 : 2);
+  const int64_t total = a_q.size(0), k = a_q.size(1), l = offsets ? b_q.size(0) : 1, n = b_q.size(-2);
+  need(a_sf, "a_sf", kF32, {blocks_of(k), pitch_of(total)});
+  if (offsets) {
+    need(b_q, "b_q", kE4m3, {l, n, k});
+    need(b_sf, "b_sf", kF32, {l, blocks_of(n), blocks_of(k)});
+    need(*offsets, "group_offsets", kI32, {l});
+    need(*rows, "group_rows", kI32, {l});
+    if (row_scale) need(*row_scale, "row_scale", kF32, {total});
+  } else {
+    need(b_q, "b_q", kE4m3, {n, k});
+    need(b_sf, "b_sf", kF32, {blocks_of(n), blocks_of(k)});
+  }
+  if (out) {
+    need(*out, "out", kFloats, {total, n});
+    if (out_type >= 0 && out->scalar_type() != kOutTypes[out_type])
+      value_error(std::string("out has dtype ") + c10::toString(out->scalar_type()) + ", expected " + c10::toString(kOutTypes[out_type]));
+    out_type = dt3(*out);
+  }
+  if (out_type < 0) out_type = 0;
+  one_device(a_q, {{&a_sf, "a_sf"}, {&b_q, "b_q"}, {&b_sf, "b_sf"}, {opt_ptr(offsets), "group_offsets"}, {opt_ptr(rows), "group_rows"},
+                   {opt_ptr(row_scale), "row_scale"}, {opt_ptr(out), "out"}});
+  const int ll = as_int(l, "l"), tt = as_int(total, "rows"), nn = as_int(n, "n"), kk = as_int(k, "k"), ctas = as_int(max_ctas, "max_ctas");
+  if (!out) out = empty({total, n}, kOutTypes[out_type], a_q);
+  if (!total) return *out;
+  const Lib& f = lib();
+  const OnDeviceOf on(a_q);
+  launch([&] {
+    if (!offsets)
+      return f.msc_gemm_fp8_block(ptr(a_q), ptr<float>(a_sf), ptr(b_q), ptr<float>(b_sf), out->data_ptr(), out_type, tt, nn, kk,
+                                  ctas, on.stream);
+    return f.msc_grouped_gemm_fp8_block_ragged(ptr(a_q), ptr<float>(a_sf), ptr(b_q), ptr<float>(b_sf), ptr<int32_t>(offsets),
+                                               ptr<int32_t>(rows), ptr<float>(row_scale), out->data_ptr(), out_type, ll, tt, nn, kk,
+                                               ctas, on.stream);
+  });
+  return *out;
+}
+
 // Whether a factor of the masked layer is what msc_moe_masked reads: one fp32 per expert.
 bool per_expert(const OptTensor& t, int64_t l) {
   return t && t->is_cuda() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 1 && t->size(0) == l;
@@ -687,6 +888,48 @@ PY_FUNCTION(mixed_grouped_gemm_int4, 11) {
                                tensor(a[4], "group_rows"), opt_tensor(a[5], "alpha"), integer(a[6]), opt_tensor(a[7], "workspace"),
                                opt_tensor(a[8], "out"), a[9] == Py_None ? -1 : (int)truth(a[9]), (int)integer(a[10])));
 }
+double real(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) raise();
+  return v;
+}
+// (logits, topk, bias, score, groups, topk_groups, group_top, renormalize, scale, (ids, weights) or None)
+PY_FUNCTION(moe_route_scores, 10) {
+  OptTensor ids, weights;
+  opt_pair(a[9], ids, weights);
+  msc_route_cfg cfg;
+  cfg.score = as_int(integer(a[3]), "score");
+  cfg.groups = as_int(integer(a[4]), "groups");
+  cfg.topk_groups = as_int(integer(a[5]), "topk_groups");
+  cfg.group_top = as_int(integer(a[6]), "group_top");
+  cfg.renormalize = truth(a[7]);
+  cfg.scale = (float)real(a[8]);
+  return wrap(moe_route(tensor(a[0], "logits"), integer(a[1]), opt_tensor(a[2], "bias"), cfg, ids, weights));
+}
+PY_FUNCTION(moe_route_backward, 8) {
+  return wrap(moe_route_backward(tensor(a[0], "grad_weights"), tensor(a[1], "logits"), tensor(a[2], "ids"), tensor(a[3], "weights"),
+                                 as_int(integer(a[4]), "score"), truth(a[5]), real(a[6]), opt_tensor(a[7], "out")));
+}
+PY_FUNCTION(quantize_fp8_block, 5) {
+  OptTensor q, sf;
+  opt_pair(a[4], q, sf);
+  return wrap(quantize_fp8_block(tensor(a[0], "x"), truth(a[1]), opt_tensor(a[2], "group_offsets"), opt_tensor(a[3], "group_rows"), q,
+                                 sf, false));
+}
+PY_FUNCTION(quantize_fp8_block_weight, 2) {
+  OptTensor q, sf;
+  opt_pair(a[1], q, sf);
+  return wrap(quantize_fp8_block_weight(tensor(a[0], "w"), q, sf));
+}
+PY_FUNCTION(gemm_fp8_block, 7) {
+  return wrap(gemm_fp8_block(tensor(a[0], "a_q"), tensor(a[1], "a_sf"), tensor(a[2], "b_q"), tensor(a[3], "b_sf"), std::nullopt,
+                             std::nullopt, std::nullopt, (int)integer(a[4]), opt_tensor(a[5], "out"), integer(a[6])));
+}
+PY_FUNCTION(ragged_grouped_gemm_fp8_block, 10) {
+  return wrap(gemm_fp8_block(tensor(a[0], "a_q"), tensor(a[1], "a_sf"), tensor(a[2], "b_q"), tensor(a[3], "b_sf"),
+                             tensor(a[4], "group_offsets"), tensor(a[5], "group_rows"), opt_tensor(a[6], "row_scale"),
+                             (int)integer(a[7]), opt_tensor(a[8], "out"), integer(a[9])));
+}
 // -> the result, or None where the separate steps have to be taken
 PY_FUNCTION(moe_masked, 14) {
   const OptTensor out =
@@ -823,6 +1066,12 @@ PyMethodDef kMethods[] = {METHOD(masked_grouped_gemm),
                           METHOD(ragged_grouped_gemm_bf16),
                           METHOD(mixed_grouped_gemm_int4),
                           METHOD(moe_masked),
+                          METHOD(moe_route_scores),
+                          METHOD(moe_route_backward),
+                          METHOD(quantize_fp8_block),
+                          METHOD(quantize_fp8_block_weight),
+                          METHOD(gemm_fp8_block),
+                          METHOD(ragged_grouped_gemm_fp8_block),
                           METHOD(moe_route),
                           METHOD(moe_dispatch),
                           METHOD(moe_combine),
@@ -892,6 +1141,47 @@ Tensor op_moe_masked(const Tensor& hidden, const Tensor& w1_q, const Tensor& w1_
   return r;
 }
 
+int score_of(c10::string_view name) {
+  if (name == "softmax") return MSC_SCORE_SOFTMAX;
+  if (name == "sigmoid") return MSC_SCORE_SIGMOID;
+  value_error("score must be 'softmax' or 'sigmoid', got '" + std::string(name) + "'");
+}
+std::tuple<Tensor, Tensor> op_moe_route(const Tensor& logits, int64_t topk, c10::string_view score, const OptTensor& bias,
+                                        int64_t groups, int64_t topk_groups, int64_t group_top, bool renormalize, double scale) {
+  msc_route_cfg cfg;
+  cfg.score = score_of(score);
+  cfg.groups = as_int(groups, "groups");
+  cfg.topk_groups = as_int(topk_groups, "topk_groups");
+  cfg.group_top = as_int(group_top, "group_top");
+  cfg.renormalize = renormalize;
+  cfg.scale = (float)scale;
+  return moe_route(logits, topk, bias, cfg, std::nullopt, std::nullopt);
+}
+Tensor op_moe_route_backward(const Tensor& grad, const Tensor& logits, const Tensor& ids, const Tensor& weights,
+                             c10::string_view score, bool renormalize, double scale) {
+  return moe_route_backward(grad, logits, ids, weights, score_of(score), renormalize, scale, std::nullopt);
+}
+std::tuple<Tensor, Tensor> op_quantize_fp8_block(const Tensor& x, bool silu, const OptTensor& offsets, const OptTensor& rows) {
+  return quantize_fp8_block(x, silu, offsets, rows, std::nullopt, std::nullopt, true);
+}
+std::tuple<Tensor, Tensor> op_quantize_fp8_block_weight(const Tensor& w) { return quantize_fp8_block_weight(w, std::nullopt, std::nullopt); }
+int out_type_of(at::ScalarType t) {
+  for (int i = 0; i < 3; ++i)
+    if (kOutTypes[i] == t) return i;
+  value_error(std::string("out_dtype must be bfloat16, float16 or float32, got ") + c10::toString(t));
+}
+Tensor op_gemm_fp8_block(const Tensor& a_q, const Tensor& a_sf, const Tensor& b_q, const Tensor& b_sf, at::ScalarType out_dtype) {
+  return gemm_fp8_block(a_q, a_sf, b_q, b_sf, std::nullopt, std::nullopt, std::nullopt, out_type_of(out_dtype), std::nullopt, 0);
+}
+Tensor op_grouped_gemm_fp8_block_ragged(const Tensor& a_q, const Tensor& a_sf, const Tensor& b_q, const Tensor& b_sf,
+                                        const Tensor& offsets, const Tensor& rows, const OptTensor& row_scale, at::ScalarType out_dtype) {
+  need_dim(a_q, "a_q", 2);
+  need_dim(b_q, "b_q", 3);
+  const int out_type = out_type_of(out_dtype);
+  return gemm_fp8_block(a_q, a_sf, b_q, b_sf, offsets, rows, row_scale, out_type,
+                        at::zeros({a_q.size(0), b_q.size(1)}, a_q.options().dtype(out_dtype)), 0);
+}
+
 // The operators' schemas are in mosaicist_b200.torch_ops.
 TORCH_LIBRARY_IMPL(mosaicist_sm100a, CUDA, m) {
   m.impl("grouped_gemm_nvfp4", op_grouped_gemm_nvfp4);
@@ -904,13 +1194,20 @@ TORCH_LIBRARY_IMPL(mosaicist_sm100a, CUDA, m) {
   m.impl("gemm_f16", op_gemm_f16);
   m.impl("grouped_gemm_bf16_int4_ragged", op_grouped_gemm_bf16_int4_ragged);
   m.impl("moe_masked", op_moe_masked);
+  m.impl("moe_route", op_moe_route);
+  m.impl("moe_route_backward", op_moe_route_backward);
+  m.impl("quantize_fp8_block", op_quantize_fp8_block);
+  m.impl("quantize_fp8_block_weight", op_quantize_fp8_block_weight);
+  m.impl("gemm_fp8_block", op_gemm_fp8_block);
+  m.impl("grouped_gemm_fp8_block_ragged", op_grouped_gemm_fp8_block_ragged);
 }
 // No operator has a derivative: a backward pass through one raises.  (Without a kernel under this
 // key torch only warns and leaves the operator's share out of the gradients.)
 TORCH_LIBRARY_IMPL(mosaicist_sm100a, Autograd, m) {
   for (const char* name : {"grouped_gemm_nvfp4", "grouped_gemm_nvfp4_ragged", "quantize_nvfp4", "silu_mul_quantize_nvfp4",
                            "global_scale_for", "quantize_mxfp8", "grouped_gemm_mxfp8_ragged", "gemm_f16",
-                           "grouped_gemm_bf16_int4_ragged", "moe_masked"})
+                           "grouped_gemm_bf16_int4_ragged", "moe_masked", "moe_route", "moe_route_backward", "quantize_fp8_block",
+                           "quantize_fp8_block_weight", "gemm_fp8_block", "grouped_gemm_fp8_block_ragged"})
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
 }
 

@@ -236,3 +236,81 @@ def ragged_gemm1_swiglu_quantize(a_q, a_sf, w1_q, w1_sf, group_offsets, group_ro
     followed by the stand-alone SiLU quantiser."""
     return _host_ops.ragged_gemm1_swiglu_quantize(a_q, a_sf, w1_q, w1_sf, group_offsets, group_rows, alpha,
                                                   out_global_scale, config, out)
+
+
+_SCORES = {"softmax": _lib.SCORE_SOFTMAX, "sigmoid": _lib.SCORE_SIGMOID}
+
+
+def _score(name):
+    if name not in _SCORES:
+        raise ValueError(f"score must be one of {tuple(_SCORES)}, got {name!r}")
+    return _SCORES[name]
+
+
+def moe_route(logits, topk: int, score: str = "softmax", bias=None, groups: int = 1, topk_groups: int = 1,
+              group_top: int = 1, renormalize: bool = True, scale: float = 1.0, out=None):
+    """Experts of each token from router logits (tokens, experts) bf16 / f16 / f32: ids (tokens, topk) int32
+    in falling order and weights (tokens, topk) f32.
+
+    score: "softmax" over all experts, or "sigmoid" of each logit.  The choice goes by score + bias
+    (bias (experts,) f32, the load-balancing correction); the weights are scores alone, divided by the sum
+    of the chosen ones with `renormalize`, times `scale`.  With groups > 1 the experts form that many groups of
+    neighbours; the `topk_groups` groups whose best `group_top` (1 or 2) score + bias have the largest sum
+    take part.  Ties go to the lower expert (or group), and the order is that of 64-bit arithmetic.
+
+    A logit or bias of -inf or NaN bars its expert; where fewer than topk are left, the lowest barred ones
+    fill up, with weight 0.  `out` may carry preallocated (ids, weights).  (The reference has no routing
+    code; MegaMoE's own routing is softmax, no bias, no groups, renormalised.)"""
+    return _host_ops.moe_route_scores(logits, topk, bias, _score(score), groups, topk_groups, group_top, renormalize, scale,
+                                      out)
+
+
+def moe_route_backward(grad_weights, logits, ids, weights, score: str = "softmax", renormalize: bool = True,
+                       scale: float = 1.0, out=None):
+    """Gradient of the logits (shape and type of the logits) from grad_weights (tokens, topk) f32 and what
+    moe_route returned for these logits, score, renormalize and scale.  The choice itself has no gradient
+    (nor has the bias); ids that are not an expert are skipped."""
+    return _host_ops.moe_route_backward(grad_weights, logits, ids, weights, _score(score), renormalize, scale, out)
+
+
+def quantize_fp8_block(x, silu: bool = False, group_offsets=None, group_rows=None, out=None):
+    """(rows, k) bf16 / f16 / f32 -> (q (rows, k) e4m3 bytes, sf (ceil(k / 128), rows rounded up to 4) f32): one
+    scale per row and 128 columns, max(amax / 448, 2^-126), held by block column (structure of the
+    reference's block-scaled FP8 quantiser, flashinfer-megamoe-sm90a/quant.py:47-75).  With silu, x is
+    (rows, 2k) gate | up and silu(gate) * up, in fp32, is quantised.  k % 16 == 0.  The scale columns behind
+    `rows` are 0.  With group_offsets / group_rows only rows inside a group are written (groups may start
+    anywhere).  `out` may carry preallocated (q, sf)."""
+    return _host_ops.quantize_fp8_block(x, silu, group_offsets, group_rows, out)
+
+
+def quantize_fp8_block_weight(w, out=None):
+    """(n, k) or (l, n, k) bf16 / f16 / f32 -> (q e4m3 bytes of that shape, sf (..., ceil(n / 128),
+    ceil(k / 128)) f32): one scale per 128 x 128 block.  k % 16 == 0."""
+    return _host_ops.quantize_fp8_block_weight(w, out)
+
+
+_OUT_TYPES = {None: -1, torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+
+
+def _out_type(dtype):
+    if dtype not in _OUT_TYPES:
+        raise ValueError(f"out_dtype must be bfloat16, float16 or float32, got {dtype}")
+    return _OUT_TYPES[dtype]
+
+
+def gemm_fp8_block(a_q, a_sf, b_q, b_sf, out_dtype=None, out=None, max_ctas: int = 0):
+    """out (m, n) = dequant(a) (m, k) @ dequant(b) (n, k).T of operands as quantize_fp8_block and
+    quantize_fp8_block_weight make them: a_q (m, k), a_sf (ceil(k / 128), m rounded up to 4), b_q (n, k), b_sf
+    (ceil(n / 128), ceil(k / 128)); fp32 sums, rounded once to out_dtype (bfloat16 unless `out` or out_dtype
+    says float16 or float32).  k % 16 == 0, n % 8 == 0."""
+    return _host_ops.gemm_fp8_block(a_q, a_sf, b_q, b_sf, _out_type(out_dtype), out, max_ctas)
+
+
+def ragged_grouped_gemm_fp8_block(a_q, a_sf, b_q, b_sf, group_offsets, group_rows, row_scale=None, out_dtype=None,
+                                  out=None, max_ctas: int = 0):
+    """gemm_fp8_block over row-concatenated groups: group g owns rows [group_offsets[g], + group_rows[g]) of a_q
+    (rows_total, k) and out (rows_total, n) and the weights b_q[g] of (l, n, k), b_sf (l, ceil(n / 128),
+    ceil(k / 128)).  Groups may start anywhere; rows outside them are left as they are.  row_scale
+    (rows_total,) f32 multiplies rows before they are rounded (routing weights)."""
+    return _host_ops.ragged_grouped_gemm_fp8_block(a_q, a_sf, b_q, b_sf, group_offsets, group_rows, row_scale,
+                                                   _out_type(out_dtype), out, max_ctas)

@@ -13,6 +13,9 @@ that build graphs of torch operators (tracing, FakeTensor shape propagation) ins
     grouped_gemm_mxfp8_ragged  the MXFP8 grouped GEMM over row-concatenated groups
     gemm_f16                   the dense fp16 / bf16 problem (hopper_gemm/ref_cutedsl.py:50-74)
     grouped_gemm_bf16_int4_ragged   bf16 x int4 grouped GEMM (problems.py:75-87)
+    moe_route, moe_route_backward   expert choices from router logits (ops.moe_route), their gradient
+    quantize_fp8_block[_weight], gemm_fp8_block, grouped_gemm_fp8_block_ragged
+                               e4m3 with fp32 scales per block of 128 (ops)
     moe_masked                 the masked MoE layer, arguments of the reference's moe_masked
                                (experiments/flashinfer-megamoe-sm100a/moe.py:47-79)
 
@@ -47,7 +50,16 @@ for _schema in (
         "grouped_gemm_bf16_int4_ragged(Tensor a, Tensor b_q, Tensor scales, Tensor group_offsets, Tensor group_rows, "
         "Tensor? alpha, int group_size) -> Tensor",
         "moe_masked(Tensor hidden, Tensor w1_q, Tensor w1_sf, Tensor w1_gs, Tensor w1_alpha, Tensor w2_q, Tensor w2_sf, "
-        "Tensor w2_gs, Tensor w2_alpha, Tensor masked_m, Tensor input_global_scale, Tensor a2_global_scale) -> Tensor"):
+        "Tensor w2_gs, Tensor w2_alpha, Tensor masked_m, Tensor input_global_scale, Tensor a2_global_scale) -> Tensor",
+        "moe_route(Tensor logits, int topk, str score, Tensor? bias, int groups, int topk_groups, int group_top, "
+        "bool renormalize, float scale) -> (Tensor, Tensor)",
+        "moe_route_backward(Tensor grad_weights, Tensor logits, Tensor ids, Tensor weights, str score, bool renormalize, "
+        "float scale) -> Tensor",
+        "quantize_fp8_block(Tensor x, bool silu, Tensor? group_offsets, Tensor? group_rows) -> (Tensor, Tensor)",
+        "quantize_fp8_block_weight(Tensor w) -> (Tensor, Tensor)",
+        "gemm_fp8_block(Tensor a_q, Tensor a_sf, Tensor b_q, Tensor b_sf, ScalarType out_dtype) -> Tensor",
+        "grouped_gemm_fp8_block_ragged(Tensor a_q, Tensor a_sf, Tensor b_q, Tensor b_sf, Tensor group_offsets, "
+        "Tensor group_rows, Tensor? row_scale, ScalarType out_dtype) -> Tensor"):
     _LIBRARY.define(_schema, tags=(torch.Tag.pt2_compliant_tag,))
 
 try:
@@ -65,6 +77,12 @@ grouped_gemm_mxfp8_ragged = _OPS.grouped_gemm_mxfp8_ragged
 gemm_f16 = _OPS.gemm_f16
 grouped_gemm_bf16_int4_ragged = _OPS.grouped_gemm_bf16_int4_ragged
 moe_masked = _OPS.moe_masked
+moe_route = _OPS.moe_route
+moe_route_backward = _OPS.moe_route_backward
+quantize_fp8_block = _OPS.quantize_fp8_block
+quantize_fp8_block_weight = _OPS.quantize_fp8_block_weight
+gemm_fp8_block = _OPS.gemm_fp8_block
+grouped_gemm_fp8_block_ragged = _OPS.grouped_gemm_fp8_block_ragged
 
 
 def _fake(name):
@@ -128,3 +146,41 @@ def _(a, b_q, scales, group_offsets, group_rows, alpha, group_size):
 def _(hidden, w1_q, w1_sf, w1_gs, w1_alpha, w2_q, w2_sf, w2_gs, w2_alpha, masked_m, input_global_scale,
       a2_global_scale):
     return hidden.new_empty(hidden.shape, dtype=torch.bfloat16)
+
+
+@_fake("moe_route")
+def _(logits, topk, score, bias, groups, topk_groups, group_top, renormalize, scale):
+    shape = (logits.shape[0], topk)
+    return logits.new_empty(shape, dtype=torch.int32), logits.new_empty(shape, dtype=torch.float32)
+
+
+@_fake("moe_route_backward")
+def _(grad_weights, logits, ids, weights, score, renormalize, scale):
+    return logits.new_empty(logits.shape)
+
+
+def _blocks(n):
+    return (n + 127) // 128
+
+
+@_fake("quantize_fp8_block")
+def _(x, silu, group_offsets, group_rows):
+    rows, k = x.shape
+    k = k // 2 if silu else k
+    return x.new_empty((rows, k), dtype=torch.uint8), x.new_empty((_blocks(k), (rows + 3) // 4 * 4), dtype=torch.float32)
+
+
+@_fake("quantize_fp8_block_weight")
+def _(w):
+    scales = (*w.shape[:-2], _blocks(w.shape[-2]), _blocks(w.shape[-1]))
+    return w.new_empty(w.shape, dtype=torch.uint8), w.new_empty(scales, dtype=torch.float32)
+
+
+@_fake("gemm_fp8_block")
+def _(a_q, a_sf, b_q, b_sf, out_dtype):
+    return a_q.new_empty((a_q.shape[0], b_q.shape[0]), dtype=out_dtype)
+
+
+@_fake("grouped_gemm_fp8_block_ragged")
+def _(a_q, a_sf, b_q, b_sf, group_offsets, group_rows, row_scale, out_dtype):
+    return a_q.new_empty((a_q.shape[0], b_q.shape[1]), dtype=out_dtype)

@@ -1,0 +1,196 @@
+"""Refusals of the routing and FP8 block operators: by the host path on FakeTensors (device and shape, no
+memory) and by the C ABI itself, which refuses before anything is launched.  No GPU work happens here."""
+
+import ctypes
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from mosaicist_b200 import _lib, ops
+
+BF16, F16, F32, U8, I32, E4 = torch.bfloat16, torch.float16, torch.float32, torch.uint8, torch.int32, torch.float8_e4m3fn
+
+
+@pytest.fixture
+def fake():
+    with FakeTensorMode():
+        yield
+
+
+def _t(*shape, dtype=F32, device="cuda"):
+    return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _refused(call, *args):
+    for a in args:
+        with pytest.raises(ValueError):
+            call(a)
+
+
+def test_route_arguments(fake):
+    x = _t(16, 64)
+    _refused(lambda v: ops.moe_route(v, 4), _t(16, 64, device="cpu"), _t(16, 64, dtype=torch.float64), _t(64, 16).t(), _t(64),
+             _t(2, 16, 64))
+    _refused(lambda v: ops.moe_route(x, v), 0, -1, 65)
+    _refused(lambda v: ops.moe_route(x, 4, bias=v), _t(63), _t(64, dtype=BF16), _t(64, device="cpu"), _t(1, 64), _t(128)[::2])
+    _refused(lambda v: ops.moe_route(x, 4, score=v), "tanh", None, 0)
+    _refused(lambda v: ops.moe_route(x, 4, groups=v), -1)
+    ids, w = _t(16, 4, dtype=I32), _t(16, 4)
+    _refused(lambda v: ops.moe_route(x, 4, out=v), (_t(16, 3, dtype=I32), w), (_t(16, 4, dtype=torch.int64), w), (ids, _t(16, 4, dtype=BF16)),
+             (ids, _t(4, 16).t()), (ids,), (ids.cpu(), w))
+    _refused(lambda v: ops.moe_route(x, 4, out=v), (ids, _t(16, 4, device="cuda:1")))
+
+
+def test_route_backward_arguments(fake):
+    g, x, ids, w = _t(16, 4), _t(16, 64), _t(16, 4, dtype=I32), _t(16, 4)
+    _refused(lambda v: ops.moe_route_backward(v, x, ids, w), _t(16, 3), _t(15, 4), _t(16, 4, dtype=BF16), _t(4, 16).t(), _t(16, 4, device="cpu"))
+    _refused(lambda v: ops.moe_route_backward(g, v, ids, w), _t(15, 64), _t(16, 64, dtype=torch.float64), _t(64, 16).t(), _t(16))
+    _refused(lambda v: ops.moe_route_backward(g, x, v, w), _t(16, 4, dtype=torch.int64), _t(16, 3, dtype=I32), _t(16, dtype=I32))
+    _refused(lambda v: ops.moe_route_backward(g, x, ids, v), _t(16, 3), _t(16, 4, dtype=F16))
+    _refused(lambda v: ops.moe_route_backward(g, x, ids, w, out=v), _t(16, 63), _t(16, 64, dtype=BF16), _t(64, 16).t())
+    _refused(lambda v: ops.moe_route_backward(g, x, ids, w, score=v), "none")
+
+
+def test_quantizer_arguments(fake):
+    x = _t(100, 272, dtype=BF16)
+    q, sf = _t(100, 272, dtype=U8), _t(3, 100)
+    _refused(lambda v: ops.quantize_fp8_block(v), x.cpu(), _t(272, 100).t(), _t(100), _t(100, 272, dtype=U8), _t(4, 100, 272))
+    _refused(lambda v: ops.quantize_fp8_block(v, silu=True), _t(100, 271))
+    _refused(lambda v: ops.quantize_fp8_block(x, out=v), (q[:99], sf), (q, _t(2, 100)), (q, _t(3, 104)), (q, _t(3, 100, dtype=BF16)),
+             (_t(100, 272, dtype=BF16), sf), (q,), (q, _t(100, 3).t()))
+    offs, rows = _t(4, dtype=I32), _t(4, dtype=I32)
+    _refused(lambda v: ops.quantize_fp8_block(x, group_offsets=v, group_rows=rows), None, _t(3, dtype=I32), _t(4, dtype=torch.int64), _t(4, 1, dtype=I32))
+    _refused(lambda v: ops.quantize_fp8_block(x, group_offsets=offs, group_rows=v), None, _t(5, dtype=I32), offs.cpu())
+    _refused(lambda v: ops.quantize_fp8_block(x, group_offsets=v, group_rows=v), _t(0, dtype=I32))
+    w = _t(260, 272)
+    _refused(lambda v: ops.quantize_fp8_block_weight(v), w.cpu(), w.t(), _t(260), _t(1, 2, 260, 272), _t(260, 272, dtype=torch.float64))
+    wq, wsf = _t(260, 272, dtype=U8), _t(3, 3)
+    _refused(lambda v: ops.quantize_fp8_block_weight(w, out=v), (wq, _t(2, 3)), (wq[:259], wsf), (wq, _t(1, 3, 3)), (wq, wsf.cpu()))
+
+
+def test_product_arguments(fake):
+    a, sa, b, sb = _t(50, 272, dtype=U8), _t(3, 52), _t(264, 272, dtype=E4), _t(3, 3)
+    call = ops.gemm_fp8_block
+    _refused(lambda v: call(v, sa, b, sb), _t(50, 256, dtype=U8), _t(50, 272, dtype=BF16), a.cpu(), _t(272, 50, dtype=U8).t(), _t(272, dtype=U8))
+    _refused(lambda v: call(a, v, b, sb), _t(3, 50), _t(52, 3).t(), _t(2, 52), _t(3, 52, dtype=BF16))
+    _refused(lambda v: call(a, sa, v, sb), _t(264, 256, dtype=U8), _t(1, 264, 272, dtype=U8), _t(272, 264, dtype=U8).t())
+    _refused(lambda v: call(a, sa, b, v), _t(2, 3), _t(3, 2), _t(3, 3, dtype=F16), _t(1, 3, 3))
+    _refused(lambda v: call(a, sa, b, sb, out=v), _t(50, 263), _t(50, 264, dtype=U8), _t(264, 50).t(), _t(50, 264, device="cpu"))
+    _refused(lambda v: call(a, sa, b, sb, out_dtype=v), torch.float64, U8, "bf16")
+    _refused(lambda v: call(a, sa, b, sb, out_dtype=BF16, out=v), _t(50, 264))
+    _refused(lambda v: call(a, sa, b, sb, max_ctas=v), -1)
+    b3, sb3, offs, rows = _t(4, 264, 272, dtype=U8), _t(4, 3, 3), _t(4, dtype=I32), _t(4, dtype=I32)
+    g = ops.ragged_grouped_gemm_fp8_block
+    _refused(lambda v: g(a, sa, v, sb3, offs, rows), b, _t(3, 264, 272, dtype=U8), _t(4, 264, 288, dtype=U8))
+    _refused(lambda v: g(a, sa, b3, v, offs, rows), sb, _t(3, 3, 3))
+    _refused(lambda v: g(a, sa, b3, sb3, v, rows), _t(3, dtype=I32), _t(4, dtype=torch.int64), _t(4, dtype=I32, device="cpu"))
+    _refused(lambda v: g(a, sa, b3, sb3, offs, v), _t(3, dtype=I32), _t(8, dtype=I32)[::2])
+    _refused(lambda v: g(a, sa, b3, sb3, offs, rows, v), _t(49), _t(50, dtype=BF16), _t(50, 1))
+    for arg in (sa, b3, sb3, offs, rows):
+        args = [a, sa, b3, sb3, offs, rows]
+        i = next(j for j, v in enumerate(args) if v is arg)
+        args[i] = _t(*arg.shape, dtype=arg.dtype, device="cuda:1")
+        with pytest.raises(ValueError, match="expected cuda:0"):
+            g(*args)
+
+
+# ---- the C ABI -----------------------------------------------------------------------------
+
+P = 4096      # a pointer that nothing follows: the calls below are refused
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from mosaicist_b200 import build
+
+    build.build()
+    return _lib.load()
+
+
+def _cfg(score=0, groups=1, topk_groups=1, group_top=1, renormalize=1, scale=1.0):
+    return _lib.RouteCfg(score, groups, topk_groups, group_top, renormalize, scale)
+
+
+def _route(lib, logits=P, dtype=1, bias=None, ids=P, w=P, tokens=8, experts=64, topk=4, cfg=None):
+    return lib.msc_moe_route(logits, dtype, bias, ids, w, tokens, experts, topk, ctypes.byref(cfg or _cfg()), None)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(logits=None), dict(ids=None), dict(w=None), dict(dtype=3), dict(dtype=-1), dict(tokens=-1), dict(experts=0), dict(experts=1025),
+    dict(topk=0), dict(topk=33), dict(topk=65), dict(logits=P + 2), dict(logits=P + 1, dtype=0), dict(bias=P + 2), dict(ids=P + 1), dict(w=P + 2),
+    dict(cfg=_cfg(score=2)), dict(cfg=_cfg(groups=0)), dict(cfg=_cfg(groups=3)), dict(cfg=_cfg(groups=64)), dict(cfg=_cfg(groups=8, topk_groups=0)),
+    dict(cfg=_cfg(groups=8, topk_groups=9)), dict(cfg=_cfg(group_top=0)), dict(cfg=_cfg(group_top=3)),
+    dict(cfg=_cfg(groups=32, group_top=2), experts=32), dict(cfg=_cfg(groups=16, topk_groups=1), topk=5), dict(cfg=_cfg(scale=0.0)),
+    dict(cfg=_cfg(scale=-1.0)), dict(cfg=_cfg(scale=float("nan"))), dict(cfg=_cfg(scale=float("inf"))),
+    dict(cfg=_cfg(groups=31, topk_groups=4), experts=31 * 33), dict(cfg=_cfg(groups=20, topk_groups=4), experts=20 * 40)])
+def test_route_refusals(lib, kw):
+    assert _route(lib, **kw) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
+    assert lib.msc_last_error()
+
+
+def test_empty_calls_do_nothing(lib):
+    assert _route(lib, tokens=0) == _lib.OK
+    assert lib.msc_moe_route_backward(P, P, 1, P, P, P, 0, 64, 4, 0, 1, 1.0, None) == _lib.OK
+    assert lib.msc_fp8_block_quantize(P, 0, 0, None, None, P, P, 0, 0, 128, None) == _lib.OK
+    assert lib.msc_gemm_fp8_block(P, P, P, P, P, 0, 0, 128, 128, 0, None) == _lib.OK
+
+
+@pytest.mark.parametrize("args", [
+    (None, P, 1, P, P, P, 8, 64, 4, 0, 1, 1.0), (P, None, 1, P, P, P, 8, 64, 4, 0, 1, 1.0), (P, P, 1, None, P, P, 8, 64, 4, 0, 1, 1.0),
+    (P, P, 1, P, None, P, 8, 64, 4, 0, 1, 1.0), (P, P, 1, P, P, None, 8, 64, 4, 0, 1, 1.0), (P, P, 5, P, P, P, 8, 64, 4, 0, 1, 1.0),
+    (P, P, 1, P, P, P, -8, 64, 4, 0, 1, 1.0), (P, P, 1, P, P, P, 8, 2000, 4, 0, 1, 1.0), (P, P, 1, P, P, P, 8, 64, 40, 0, 1, 1.0),
+    (P, P, 1, P, P, P, 8, 64, 4, 2, 1, 1.0), (P, P, 1, P, P, P, 8, 64, 4, 0, 1, 0.0), (P + 1, P, 1, P, P, P, 8, 64, 4, 0, 1, 1.0),
+    (P, P, 1, P, P, P + 2, 8, 64, 4, 0, 1, 1.0)])
+def test_route_backward_refusals(lib, args):
+    assert lib.msc_moe_route_backward(*args, None) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
+
+
+@pytest.mark.parametrize("args", [
+    (None, 0, 0, None, None, P, P, 0, 8, 128), (P, 0, 0, None, None, None, P, 0, 8, 128), (P, 0, 0, None, None, P, None, 0, 8, 128),
+    (P, 0, 0, P, None, P, P, 1, 8, 128), (P, 0, 0, None, P, P, P, 1, 8, 128), (P, 0, 0, P, P, P, P, 0, 8, 128), (P, 0, 0, None, None, P, P, 0, -1, 128),
+    (P, 0, 0, None, None, P, P, 0, 8, 0), (P, 0, 0, None, None, P, P, 0, 8, 120), (P, 3, 0, None, None, P, P, 0, 8, 128),
+    (P + 8, 0, 0, None, None, P, P, 0, 8, 128), (P, 0, 0, None, None, P + 8, P, 0, 8, 128), (P, 0, 0, None, None, P, P + 2, 0, 8, 128),
+    (P, 0, 0, None, None, P, P, 0, 600000, 128)])
+def test_quantizer_refusals(lib, args):
+    assert lib.msc_fp8_block_quantize(*args, None) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
+
+
+@pytest.mark.parametrize("args", [
+    (None, 0, P, P, 1, 128, 128), (P, 0, None, P, 1, 128, 128), (P, 0, P, None, 1, 128, 128), (P, 0, P, P, 0, 128, 128), (P, 0, P, P, 1, 0, 128),
+    (P, 0, P, P, 1, 128, 0), (P, 0, P, P, 1, 128, 100), (P, 7, P, P, 1, 128, 128), (P + 4, 0, P, P, 1, 128, 128), (P, 0, P + 4, P, 1, 128, 128),
+    (P, 0, P, P + 1, 1, 128, 128), (P, 0, P, P, 70000, 128, 128)])
+def test_weight_quantizer_refusals(lib, args):
+    assert lib.msc_fp8_block_quantize_weight(*args, None) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
+
+
+@pytest.mark.parametrize("args", [
+    (None, P, P, P, P, 0, 8, 128, 128, 0), (P, None, P, P, P, 0, 8, 128, 128, 0), (P, P, None, P, P, 0, 8, 128, 128, 0),
+    (P, P, P, None, P, 0, 8, 128, 128, 0), (P, P, P, P, None, 0, 8, 128, 128, 0), (P, P, P, P, P, 3, 8, 128, 128, 0),
+    (P, P, P, P, P, 0, -1, 128, 128, 0), (P, P, P, P, P, 0, 8, 0, 128, 0), (P, P, P, P, P, 0, 8, 128, 0, 0), (P, P, P, P, P, 0, 8, 100, 128, 0),
+    (P, P, P, P, P, 0, 8, 128, 100, 0), (P, P, P, P, P, 0, 8, 128, 128, -2), (P + 8, P, P, P, P, 0, 8, 128, 128, 0), (P, P + 4, P, P, P, 0, 8, 128, 128, 0),
+    (P, P, P + 1, P, P, 0, 8, 128, 128, 0), (P, P, P, P + 2, P, 0, 8, 128, 128, 0), (P, P, P, P, P + 8, 0, 8, 128, 128, 0)])
+def test_product_refusals(lib, args):
+    assert lib.msc_gemm_fp8_block(*args, None) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
+
+
+@pytest.mark.parametrize("args", [
+    (P, P, P, P, None, P, None, P, 0, 2, 8, 128, 128, 0), (P, P, P, P, P, None, None, P, 0, 2, 8, 128, 128, 0), (P, P, P, P, P, P, None, P, 0, 0, 8, 128, 128, 0),
+    (P, P, P, P, P, P, P + 2, P, 0, 2, 8, 128, 128, 0), (P, P, P, P, P, P, None, P, 0, 1 << 20, 8, 1 << 12, 128, 0)])
+def test_grouped_product_refusals(lib, args):
+    assert lib.msc_grouped_gemm_fp8_block_ragged(*args, None) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
+
+
+def test_operators_can_be_traced(fake):
+    import mosaicist_b200.torch_ops as O
+
+    x = _t(10, 544, dtype=BF16)
+    q, sf = O.quantize_fp8_block(x, True, None, None)
+    assert q.shape == (10, 272) and sf.shape == (3, 12) and sf.dtype == F32
+    wq, wsf = O.quantize_fp8_block_weight(_t(2, 136, 272))
+    assert wq.shape == (2, 136, 272) and wsf.shape == (2, 2, 3)
+    assert O.gemm_fp8_block(q, sf, wq[0], wsf[0], F16).dtype == F16
+    assert O.grouped_gemm_fp8_block_ragged(q, sf, wq, wsf, _t(2, dtype=I32), _t(2, dtype=I32), None, F32).shape == (10, 136)
+    ids, w = O.moe_route(_t(10, 64), 4, "sigmoid", None, 1, 1, 1, True, 1.0)
+    assert ids.dtype == I32 and w.shape == (10, 4)
+    assert O.moe_route_backward(w, _t(10, 64, dtype=F16), ids, w, "sigmoid", True, 1.0).dtype == F16

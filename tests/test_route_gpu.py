@@ -1,0 +1,277 @@
+"""Expert routing (ops.moe_route, ops.moe_route_backward) against the oracle in 64 bits."""
+
+import itertools
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import route as R
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+EPS = {"f32": 2.0 ** -24, "bf16": 2.0 ** -8, "f16": 2.0 ** -11}
+# Weights: expf is off by at most 2 ulp (2^-22), each of the other roundings by 2^-24: the chosen scores'
+# sum (up to five additions over lanes), two quotients, the scale.  A softmax that is not renormalised
+# divides by a sum of terms that are off by 2^-22 + |x - max| 2^-24 (|x - max| < 20 here matters: e^-20
+# of the largest), and up to 37 additions.
+W_TOL = 2.0 ** -22 * 2 + 10 * 2.0 ** -24
+W_TOL_SUM = 2.0 ** -22 * 2 + (20 + 37 + 10) * 2.0 ** -24
+
+
+def _run(logits, topk, dtype="f32", bias=None, **kw):
+    from mosaicist_b200 import ops
+
+    x = torch.from_numpy(logits.astype(np.float32)).to(DT[dtype]).cuda()
+    b = None if bias is None else torch.from_numpy(bias.astype(np.float32)).cuda()
+    ids, w = ops.moe_route(x, topk, bias=b, **kw)
+    seen = x.float().cpu().numpy()
+    return seen, ids, w
+
+
+def _check(logits, topk, dtype="f32", bias=None, score="softmax", renormalize=True, **kw):
+    seen, ids, w = _run(logits, topk, dtype, bias, score=score, renormalize=renormalize, **kw)
+    want_ids, want_w = R.route(seen, topk, score, None if bias is None else bias.astype(np.float32), renormalize=renormalize, **kw)
+    assert ids.dtype == torch.int32 and w.dtype == torch.float32
+    assert np.array_equal(ids.cpu().numpy(), want_ids)
+    tol = W_TOL_SUM if score == "softmax" and not renormalize else W_TOL
+    # (an absolute 2^-126: e^x below that is flushed to zero)
+    assert (np.abs(w.cpu().numpy() - want_w) <= tol * want_w + 2.0 ** -126 * kw.get("scale", 1.0)).all()
+    return seen, ids, w
+
+
+SHAPES = [  # experts, topk, groups, topk_groups, group_top
+    (1, 1, 1, 1, 1), (2, 1, 1, 1, 1), (31, 5, 1, 1, 1), (61, 4, 1, 1, 1), (64, 32, 1, 1, 1), (160, 6, 8, 3, 1),
+    (160, 6, 8, 3, 2), (256, 8, 8, 4, 2), (288, 8, 32, 4, 2), (384, 8, 1, 1, 1), (100, 7, 4, 4, 2), (512, 10, 16, 5, 2),
+    (640, 3, 2, 1, 1), (1000, 8, 1, 1, 1), (1024, 32, 32, 7, 2), (12, 2, 4, 2, 1)]
+
+
+@pytest.mark.parametrize("score,biased,renormalize", list(itertools.product(["softmax", "sigmoid"], [False, True], [True, False])))
+@pytest.mark.parametrize("E,k,G,tg,gt", SHAPES)
+def test_route(E, k, G, tg, gt, score, biased, renormalize):
+    rng = np.random.default_rng([E, k, G, biased])
+    T = 131
+    bias = rng.standard_normal(E) * 0.1 if biased else None
+    for dtype in DT:
+        _check(rng.standard_normal((T, E)) * 1.5, k, dtype, bias, score=score, renormalize=renormalize, groups=G, topk_groups=tg,
+               group_top=gt, scale=2.5)
+
+
+@pytest.mark.parametrize("T", [1, 3, 4, 5, 8192])
+def test_token_counts(T):
+    rng = np.random.default_rng(T)
+    _check(rng.standard_normal((T, 64)), 4, bias=rng.standard_normal(64) * 0.1, score="sigmoid")
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [(1, 1, 1), (4, 2, 2)])
+def test_keys_closer_than_fp32_tells_apart(score, groups):
+    """Scores and biases whose sums differ by 1e-9 to 1e-6 from one expert to the next, in shuffled order:
+    the order is that of the sums in 64 bits."""
+    G, tg, gt = groups
+    rng = np.random.default_rng(5)
+    T, E = 64, 64
+    for gap in (1e-9, 1e-8, 1e-7, 1e-6):
+        logits = rng.standard_normal((T, E)).astype(np.float32)
+        # one bias serves all tokens, so each token's logits are set from the key it is to have
+        bias = (rng.standard_normal(E) * 0.05).astype(np.float32)
+        for t in range(T):
+            p = 0.3 + rng.permutation(E) * gap - bias.astype(np.float64)      # scores wanted
+            logits[t] = np.log(p / (1 - p)) if score == "sigmoid" else np.log(p)
+        _check(logits, 8, bias=bias, score=score, groups=G, topk_groups=tg, group_top=gt)
+
+
+def test_ties_go_to_the_lower_expert_and_group():
+    from mosaicist_b200 import ops
+
+    x = torch.zeros(5, 64, device="cuda")
+    x[1, 40] = x[1, 7] = 3.0
+    for kw in (dict(), dict(score="sigmoid"), dict(bias=torch.zeros(64, device="cuda")),
+               dict(score="sigmoid", bias=torch.full((64,), 0.25, device="cuda"))):
+        ids, w = ops.moe_route(x, 3, **kw)
+        assert ids[0].tolist() == [0, 1, 2] and ids[1].tolist() == [7, 40, 0]
+        assert torch.equal(w[0], torch.full((3,), 1 / 3, device="cuda"))
+        ids, _ = ops.moe_route(x, 3, groups=8, topk_groups=2, group_top=2, **kw)
+        assert ids[0].tolist() == [0, 1, 2] and ids[1].tolist() == [7, 40, 0]
+    # saturated scores are equal although the logits are not: with a bias the sums tie, without one the
+    # logits decide
+    x = torch.full((1, 8), 40.0, device="cuda")
+    x[0, 5] = 60.0
+    assert ops.moe_route(x, 1, score="sigmoid")[0].item() == 5
+    assert ops.moe_route(x, 1, score="sigmoid", bias=torch.zeros(8, device="cuda"))[0].item() == 0
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("renormalize", [False, True])
+def test_barred_experts(score, biased, renormalize):
+    """Logits of -inf and NaN, biases of -inf: barred; rows that leave fewer than topk, one, or nothing."""
+    rng = np.random.default_rng(11)
+    T, E = 40, 96
+    x = rng.standard_normal((T, E))
+    bias = rng.standard_normal(E) * 0.1 if biased else None
+    if biased:
+        bias[17] = -np.inf
+        bias[18] = np.nan
+    x[0] = -np.inf
+    x[1] = np.nan
+    x[2, 1:] = -np.inf
+    x[3, :90] = -np.inf
+    x[4, 5:] = np.nan
+    x[5] = np.finfo(np.float32).min
+    x[6, ::2] = np.finfo(np.float32).min
+    x[7] = 1e4
+    x[8, 3] = 1e30
+    x[9, rng.permutation(E)[:50]] = -np.inf
+    for kw in (dict(), dict(groups=8, topk_groups=3, group_top=1), dict(groups=8, topk_groups=3, group_top=2)):
+        seen, ids, w = _check(x, 7, "f32", bias, score=score, renormalize=renormalize, **kw)
+        got = ids.cpu().numpy()
+        assert all(len(set(r)) == 7 for r in got.tolist()) and got.min() >= 0 and got.max() < E
+        assert torch.isfinite(w).all() and (w[0] == 0).all() and (w[1] == 0).all()
+
+
+def test_infinite_logits():
+    x = np.zeros((3, 40))
+    x[0, 9] = np.inf
+    x[1, [4, 30]] = np.inf
+    x[2] = np.inf
+    for score in ("softmax", "sigmoid"):
+        for bias in (None, np.zeros(40)):
+            _check(x, 3, bias=bias, score=score, renormalize=False)
+
+
+def test_infinite_bias_comes_first():
+    x = np.random.default_rng(0).standard_normal((16, 64))
+    bias = np.zeros(64)
+    bias[[50, 60]] = np.inf
+    _, ids, _ = _run(x, 4, bias=bias, score="sigmoid")
+    assert (ids[:, :2].cpu().numpy() == [50, 60]).all()
+
+
+@pytest.mark.parametrize("score,renormalize", list(itertools.product(["softmax", "sigmoid"], [True, False])))
+@pytest.mark.parametrize("E,k", [(1, 1), (33, 4), (61, 4), (160, 6), (256, 8), (1024, 32)])
+def test_backward(E, k, score, renormalize):
+    from mosaicist_b200 import ops
+
+    rng = np.random.default_rng([E, k])
+    T, scale = 77, 2.5
+    for dtype in DT:
+        x = torch.from_numpy(rng.standard_normal((T, E)).astype(np.float32)).to(DT[dtype]).cuda()
+        ids, w = ops.moe_route(x, k, score=score, renormalize=renormalize, scale=scale)
+        g = torch.from_numpy(rng.standard_normal((T, k)).astype(np.float32)).cuda()
+        got = ops.moe_route_backward(g, x, ids, w, score=score, renormalize=renormalize, scale=scale)
+        assert got.dtype == x.dtype and got.shape == x.shape
+        xs, i, ws, gs = x.float().cpu().numpy(), ids.cpu().numpy(), w.cpu().numpy(), g.cpu().numpy()
+        want = R.route_backward(gs, xs, i, ws, score, renormalize, scale)
+        # sum g w and what it meets: the terms' magnitudes times (additions, exponential, quotient)
+        terms = np.abs(gs * ws).sum(1, keepdims=True)
+        part = np.take_along_axis(np.zeros_like(want), i, axis=1) + np.abs(ws) * (np.abs(gs) + terms / scale)
+        bound = np.zeros_like(want)
+        np.put_along_axis(bound, i, part, axis=1)
+        if score == "softmax" and not renormalize:
+            bound += R.scores(xs, score) * terms
+        out = got.float().cpu().numpy()
+        assert (np.abs(out - want) <= EPS[dtype] * np.abs(want) + 80 * 2.0 ** -24 * bound + (2.0 ** -25 if dtype == "f16" else 0)).all()
+
+
+@pytest.mark.parametrize("score,renormalize", list(itertools.product(["softmax", "sigmoid"], [True, False])))
+def test_backward_against_differences(score, renormalize):
+    """The kernel's gradient against central differences of the weights in 64 bits, the choice held."""
+    from mosaicist_b200 import ops
+
+    rng = np.random.default_rng(3)
+    T, E, k, scale, h = 5, 24, 4, 1.5, 1e-5
+    x = rng.standard_normal((T, E)).astype(np.float32)
+    g = rng.standard_normal((T, k)).astype(np.float32)
+    xt = torch.from_numpy(x).cuda()
+    ids, w = ops.moe_route(xt, k, score=score, renormalize=renormalize, scale=scale)
+    got = ops.moe_route_backward(torch.from_numpy(g).cuda(), xt, ids, w, score=score, renormalize=renormalize, scale=scale).cpu().numpy()
+    i, x64 = ids.cpu().numpy(), x.astype(np.float64)
+    for e in range(E):
+        d = np.zeros((T, E))
+        d[:, e] = h
+        diff = (R.weights_of(x64 + d, i, score, renormalize, scale) - R.weights_of(x64 - d, i, score, renormalize, scale)) / (2 * h)
+        # h^2 / 6 of the third derivative (below 1 here) and fp32's share of the result
+        assert np.abs(got[:, e] - (g * diff).sum(1)).max() <= 4 * scale * np.abs(g).max() * (h * h + 80 * 2.0 ** -24)
+
+
+def test_backward_of_barred_and_repeated_ids():
+    from mosaicist_b200 import ops
+
+    x = torch.randn(6, 40, device="cuda")
+    x[0] = -torch.inf
+    x[1, 2:] = -torch.inf
+    for score, renorm in itertools.product(("softmax", "sigmoid"), (True, False)):
+        ids, w = ops.moe_route(x, 4, score=score, renormalize=renorm)
+        g = torch.randn(6, 4, device="cuda")
+        g[0] = torch.inf                   # weights of 0 do not move
+        got = ops.moe_route_backward(g, x, ids, w, score=score, renormalize=renorm)
+        want = R.route_backward(g.cpu().numpy(), x.cpu().numpy(), ids.cpu().numpy(), w.cpu().numpy(), score, renorm, 1.0)
+        assert torch.isfinite(got).all() and (got[0] == 0).all()
+        assert np.abs(got.cpu().numpy() - want).max() <= 80 * 2.0 ** -24 * 16
+    # an id twice collects both shares; ids that are no expert are skipped
+    ids = torch.tensor([[3, 3, 7, 0]] * 6, dtype=torch.int32, device="cuda")
+    w = torch.full((6, 4), 0.25, device="cuda")
+    x = torch.randn(6, 40, device="cuda")
+    got = ops.moe_route_backward(g.nan_to_num(1, 1, 1), x, ids, w, score="sigmoid", renormalize=False)
+    want = R.route_backward(g.nan_to_num(1, 1, 1).cpu().numpy(), x.cpu().numpy(), ids.cpu().numpy(), w.cpu().numpy(), "sigmoid", False, 1.0)
+    assert np.abs(got.cpu().numpy() - want).max() <= 80 * 2.0 ** -24 * 16
+    ids[:, 3] = -1
+    ids[:, 2] = 40
+    got = ops.moe_route_backward(g.nan_to_num(1, 1, 1), x, ids, w, score="sigmoid", renormalize=False)
+    assert (got[:, :3] == 0).all() and (got[:, 4:] == 0).all() and (got[:, 3] != 0).all()
+
+
+def test_out_buffers_streams_and_graphs():
+    from mosaicist_b200 import ops
+
+    x, b = torch.randn(300, 128, device="cuda"), torch.randn(128, device="cuda") * 0.1
+    kw = dict(score="sigmoid", bias=b, groups=4, topk_groups=2, group_top=2)
+    want = ops.moe_route(x, 6, **kw)
+    out = (torch.empty(300, 6, dtype=torch.int32, device="cuda"), torch.empty(300, 6, device="cuda"))
+    got = ops.moe_route(x, 6, out=out, **kw)
+    assert got[0].data_ptr() == out[0].data_ptr() and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        again = ops.moe_route(x, 6, **kw)
+        grad = ops.moe_route_backward(again[1], x, *again, score="sigmoid")
+    s.synchronize()
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        held = ops.moe_route(x, 6, **kw)
+        held_grad = ops.moe_route_backward(held[1], x, *held, score="sigmoid")
+    x.copy_(x.flip(0))
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held[0], want[0].flip(0)) and torch.equal(held[1], want[1].flip(0))
+    assert torch.equal(held_grad, grad.flip(0))
+    assert ops.moe_route(x[:0], 6, **kw)[0].shape == (0, 6)
+    assert ops.moe_route_backward(want[1][:0], x[:0], want[0][:0], want[1][:0]).shape == (0, 128)
+
+
+def test_torch_operators():
+    import mosaicist_b200.torch_ops as T
+    from mosaicist_b200 import ops
+
+    x, b = torch.randn(33, 64, device="cuda"), torch.randn(64, device="cuda") * 0.1
+    got = T.moe_route(x, 4, "sigmoid", b, 8, 3, 2, True, 2.0)
+    want = ops.moe_route(x, 4, "sigmoid", b, 8, 3, 2, True, 2.0)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    d = T.moe_route_backward(got[1], x, *got, "sigmoid", True, 2.0)
+    assert torch.equal(d, ops.moe_route_backward(got[1], x, *got, score="sigmoid", scale=2.0))
+
+
+def test_the_layers_own_routing_is_the_plain_case():
+    """msc_moe_route_topk and moe_route with its defaults make the same choices."""
+    from mosaicist_b200 import _lib, ops
+
+    x = torch.randn(500, 256, device="cuda")
+    ids, w = torch.empty(500, 8, dtype=torch.int32, device="cuda"), torch.empty(500, 8, device="cuda")
+    _lib.check(_lib.load().msc_moe_route_topk(x.data_ptr(), ids.data_ptr(), w.data_ptr(), 500, 256, 8,
+                                              torch.cuda.current_stream().cuda_stream))
+    got = ops.moe_route(x, 8)
+    assert torch.equal(got[0], ids)
+    assert (got[1] - w).abs().max() <= 2e-6
