@@ -67,7 +67,7 @@ struct Fp8Smem {
   static constexpr int kBarFull = 0;
   static constexpr int kBarEmpty = kBarFull + 8 * kMaxStages;
   static constexpr int kBarAccFull = kBarEmpty + 8 * kMaxStages;
-  static constexpr int kBarAccEmpty = kBarAccFull + 8 * kSlots;
+  static constexpr int kBarAccEmpty = kBarAccFull + 8 * kSubs * kSlots;   // full: [sub][kSlots]; empty: per accumulator
   static constexpr int kBarScaleFull = kBarAccEmpty + 8 * kSlots;        // [sub][kScales]
   static constexpr int kBarScaleEmpty = kBarScaleFull + 8 * kSubs * kScales;
   static_assert(kBarScaleEmpty + 8 * kSubs * kScales <= 1000, "barriers and flags share the first 1024 bytes");
@@ -204,8 +204,8 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       mbar_init(sbase + L::kBarFull + 8 * s, 1);
       mbar_init(sbase + L::kBarEmpty + 8 * s, 1);
     }
+    for (int s = 0; s < L::kSubs * L::kSlots; ++s) mbar_init(sbase + L::kBarAccFull + 8 * s, 1);
     for (int s = 0; s < L::kSlots; ++s) {
-      mbar_init(sbase + L::kBarAccFull + 8 * s, 1);
       mbar_init(sbase + L::kBarAccEmpty + 8 * s, 8);   // four warps of each CTA (used in the leader)
     }
     for (int s = 0; s < L::kSubs * L::kScales; ++s) {
@@ -255,7 +255,11 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     const int quad = warp & 3, sub = warp >> 2;
     const uint32_t lane_base = uint32_t(quad * 32) << 16;
     const uint32_t box = sbase + L::kOffBox + warp * L::kBoxBytes;
+    // Accumulators go round over all subs, barriers that announce them over this sub's own: a sub that sits
+    // a tile out would otherwise meet a barrier any number of phases behind, where a parity says nothing.
     uint32_t seq = 0;                  // accumulators produced before this tile
+    int af = 0;
+    uint32_t af_parity = 0;
     int ss = 0;
     uint32_t sbits = 0;
     bool ok = true;
@@ -280,8 +284,12 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
         const int sslot = sub * L::kScales + ss;
         const uint32_t now = seq0 + (uint32_t)(subs * kb), slot = now % L::kSlots;
         ok = warp_wait(sbase + L::kBarScaleFull + 8 * sslot, (sbits >> ss) & 1u, abort_flag, p.status, 6) &&
-             warp_wait(sbase + L::kBarAccFull + 8 * slot, (now / L::kSlots) & 1u, abort_flag, p.status, 4);
+             warp_wait(sbase + L::kBarAccFull + 8 * (sub * L::kSlots + af), af_parity, abort_flag, p.status, 4);
         if (!ok) break;
+        if (++af == L::kSlots) {
+          af = 0;
+          af_parity ^= 1u;
+        }
         sbits ^= 1u << ss;
         tc_fence_after_sync();
         const uint32_t tacc = tmem_base + lane_base + slot * L::kSlotCols;
@@ -445,7 +453,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       Fp8Cursor cur;
       Fp8Tile tile;
       uint32_t bits = 0, slot = 0, slot_bits = 0;
-      int s = 0;
+      int s = 0, af[L::kSubs] = {};
       bool ok = true;
       const uint64_t wdesc0 = operand_desc_sw128(sbase + L::kOffRing);
       const uint64_t tdesc0 = operand_desc_sw128(sbase + L::kOffRing + L::kW);
@@ -457,9 +465,11 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           if (!ok) break;
           bits ^= 1u << s;
           const uint32_t at = (uint32_t)s * ((uint32_t)stage_bytes >> 4);   // descriptors count 16-byte units
-          for (int h = 0; h < subs && ok; ++h) {
+#pragma unroll
+          for (int h = 0; h < L::kSubs; ++h) {
+            if (h >= subs || !ok) continue;
             ok = warp_wait(sbase + L::kBarAccEmpty + 8 * slot, ((slot_bits >> slot) & 1u) ^ 1u, abort_flag, p.status, 2);
-            if (!ok) break;
+            if (!ok) continue;
             slot_bits ^= 1u << slot;
             tc_fence_after_sync();
             const int width = tile.width(h);
@@ -470,10 +480,11 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 #pragma unroll
               for (int j = 0; j < 4; ++j)
                 tc_mma_f8_pair(tmem_base + slot * L::kSlotCols, wdesc + 2 * j, tdesc + 2 * j, idesc, j > 0 ? 1u : 0u);
-              tc_commit_pair(sbase + L::kBarAccFull + 8 * slot, 3);
+              tc_commit_pair(sbase + L::kBarAccFull + 8 * (h * L::kSlots + af[h]), 3);
               if (h == subs - 1) tc_commit_pair(sbase + L::kBarEmpty + 8 * s, 3);
             }
             __syncwarp();
+            af[h] = (af[h] + 1 == L::kSlots) ? 0 : af[h] + 1;
             slot = (slot + 1 == L::kSlots) ? 0u : slot + 1;
           }
           s = (s + 1 == stages) ? 0 : s + 1;

@@ -287,6 +287,29 @@ def test_grouped(case, scaled, exact):
         _check(got, want, mags, k, dtype, exact)
 
 
+@pytest.mark.parametrize("k", [400, 2048, 4112])
+@pytest.mark.parametrize("order", ["falling", "rising", "mixed"])
+def test_one_pair_meets_tiles_of_every_width(order, k):
+    """A single CTA pair works through tiles of one to nine units of 32 tokens: parts of the kernel sit some of them out,
+    for fewer and for more K blocks than it has accumulators."""
+    from mosaicist_b200 import ops
+
+    rows = sorted([1, 20, 33, 64, 65, 96, 100, 130, 190, 200, 256, 280, 288, 290, 330])
+    rows = rows[::-1] if order == "falling" else rows if order == "rising" else [rows[(7 * i) % 15] for i in range(15)]
+    offs, at = [], 0
+    for r in rows:
+        offs.append(at)
+        at += r
+    l, n = len(rows), 136
+    rng = np.random.default_rng(k)
+    a, sa, b, sb = _operands(rng, at, l, n, k, True)
+    want = np.concatenate([F.product(a[o:o + r], sa[:, o:o + r], b[g], sb[g])[0] for g, (o, r) in enumerate(zip(offs, rows))])
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    for ctas in (2, 4, 0):
+        got = ops.ragged_grouped_gemm_fp8_block(T(a), _dev_sf(sa), T(b), T(sb), i32(offs), i32(rows), out_dtype=torch.float32, max_ctas=ctas)
+        _check(got, want, None, k, "f32", True)
+
+
 def test_views_streams_graphs_and_float8():
     """Operands as float8 tensors and as slices at an offset; another stream; a captured call replayed on new data."""
     from mosaicist_b200 import ops
