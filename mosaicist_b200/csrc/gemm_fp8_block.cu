@@ -15,7 +15,13 @@
 // Tiles of up to 64 tokens (a decode step, what is left over of a group) exchange the roles: 256 weight rows
 // are the M side and the tokens N, rounded up to 32, so that a tile costs little more than its weights'
 // way into shared memory.  A lane then is a weight row and a register a token; the tokens' scales come by shuffle.
+//
+// A dense product with fewer tiles than half the chip has CTA pairs is split along K: clusters of two or
+// four pairs take a tile, leave their sums in shared memory and each adds up its share of the columns, in the order
+// of K.  And where the last round of a dense product's tiles would keep only a few pairs busy, its tiles are
+// taken in quarters of 64 tokens.
 #include "gemm_common.cuh"
+#include "quantize_common.cuh"
 
 #include <cuda_fp16.h>
 
@@ -32,6 +38,8 @@ struct Fp8Params {
   int out_type;              // 0 bf16, 1 f32, 2 f16
   int l, n, rows_total, pitch;
   int kblocks, nblocks;
+  int splits;                // pairs of a cluster, each with a share of K; > 1: one tile per cluster
+  int quarters_from;         // dense: tiles from this one on are taken as four of 64 tokens
 };
 
 struct Fp8Smem {
@@ -90,6 +98,17 @@ struct Fp8Tile {
 struct Fp8Cursor {
   GroupWindow<true> win;
   __device__ __forceinline__ bool seek(const Fp8Params& p, int ntiles, int t, Fp8Tile& tile) {
+    if (!p.group_rows) {   // (a tile may come out empty)
+      const int q = max(t - p.quarters_from, 0), tid = t < p.quarters_from ? t : p.quarters_from + (q >> 2);
+      const int tt = tid / ntiles;
+      tile.g = 0;
+      tile.nt = tid - tt * ntiles;
+      tile.lead = 0;
+      tile.row0 = tt * 256 + (q & 3) * 64;
+      tile.tn = min(p.rows_total - tile.row0, t < p.quarters_from ? 256 : 64);
+      shape(p, tile);
+      return tt < fp8_token_tiles(p.rows_total);
+    }
     int rows, off, first;
     if (!win.find(p.l, t, [&](int gi, int& r, int& o) { fp8_group(p, gi, r, o); },
                   [=](int r) { return fp8_token_tiles(r) * ntiles; }, tile.g, rows, off, first))
@@ -99,9 +118,12 @@ struct Fp8Cursor {
     tile.lead = tt == 0 ? (off & 3) : 0;
     tile.row0 = (off & ~3) + tt * 256;
     tile.tn = min(rows - tt * 256, 256);
+    shape(p, tile);
+    return true;
+  }
+  static __device__ __forceinline__ void shape(const Fp8Params& p, Fp8Tile& tile) {
     tile.few = tile.tn <= Fp8Smem::kFewTokens;
     tile.width = tile.few ? (tile.tn + 31) & ~31 : min((p.n - tile.nt * 256 + 31) & ~31, 256);
-    return true;
   }
 };
 
@@ -118,6 +140,22 @@ __device__ __forceinline__ void tc_mma_f8_pair(uint32_t d_tmem, uint64_t adesc, 
       : "memory");
 }
 
+__device__ __forceinline__ void st_shared_f32(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -151,7 +189,62 @@ __device__ __forceinline__ void store_box(const Fp8Params& p, uint32_t box, int 
   }
 }
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Fp8Smem::kThreads, 1)
+// The consumers' wait, made of as little code as its bound allows: it stands four times in the loop that sets the
+// kernel's pace.  A probe suspends the warp for up to 20 us.
+__device__ __forceinline__ bool wait_accumulators(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  for (int tries = 0; tries < 100000; ++tries) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, *abort_flag != 0u)) return false;
+  }
+  return false;
+}
+
+// 32 accumulator columns of a warp's 32 lanes: piece pc of the tile.
+__device__ __forceinline__ void store_piece(const Fp8Params& p, const Fp8Tile& tile, const float* v, int pc, int rank, int quad,
+                                            int lane, uint32_t box) {
+  const int mine = tile.row0 + (tile.few ? pc * 32 : rank * 128 + quad * 32);
+  const float rs = p.row_scale && mine + lane < p.rows_total ? ld_ordered(p.row_scale + mine + lane) : 1.0f;
+  const int first = tile.row0 + tile.lead, last = tile.row0 + tile.tn;
+  if (tile.few) {   // lanes are neighbouring columns of a token already
+    const int col = tile.nt * 256 + rank * 128 + quad * 32 + lane;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const float x = v[e] * __shfl_sync(0xffffffffu, rs, e);
+      if (mine + e >= first && mine + e < last && col < p.n) store_value(p, (size_t)(mine + e) * p.n + col, x);
+    }
+    return;
+  }
+  // turned around in the warp's box so that four lanes write 64 neighbouring bytes of a token
+  const int col = tile.nt * 256 + pc * 32;
+  if (col >= p.n) return;
+  if (p.out_type == 1) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {   // 16 columns are 64 bytes
+      __syncwarp();                 // the box has been read
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float* x = v + h * 16 + i * 4;
+        st_shared_v4(box + lane * Fp8Smem::kBoxPitch + i * 16, __float_as_uint(x[0] * rs), __float_as_uint(x[1] * rs),
+                     __float_as_uint(x[2] * rs), __float_as_uint(x[3] * rs));
+      }
+      __syncwarp();
+      store_box(p, box, mine, first, last, col + h * 16, 4, lane);
+    }
+  } else {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = pack_16bit(v[8 * i + 2 * j] * rs, v[8 * i + 2 * j + 1] * rs, p.out_type);
+      st_shared_v4(box + lane * Fp8Smem::kBoxPitch + i * 16, w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+    store_box(p, box, mine, first, last, col, 2, lane);
+  }
+}
+
+__global__ void __launch_bounds__(Fp8Smem::kThreads, 1)
 gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_w16,
                       const __grid_constant__ CUtensorMap tmap_t128, const __grid_constant__ CUtensorMap tmap_t32,
                       const __grid_constant__ CUtensorMap tmap_t16,
@@ -169,9 +262,13 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = __shfl_sync(0xffffffffu, cluster_ctarank(), 0);
+  const uint32_t cluster_rank = __shfl_sync(0xffffffffu, cluster_ctarank(), 0);
+  const uint32_t rank = cluster_rank & 1u;   // in the pair
   const bool leader = rank == 0;
-  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const uint16_t both = (uint16_t)(3u << (cluster_rank & ~1u));
+  const int pair = (int)blockIdx.x / (2 * p.splits), npairs = (int)gridDim.x / (2 * p.splits);   // or cluster
+  const int share = (int)(cluster_rank >> 1);
+  const int kb_lo = (int)((long long)p.kblocks * share / p.splits), kb_hi = (int)((long long)p.kblocks * (share + 1) / p.splits);
   const int ntiles = (p.n + 255) >> 8;
 
   if (threadIdx.x == 0) {
@@ -231,6 +328,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     bool ok = true;
     for (int t = pair; ok; t += npairs) {
       if (!cur.seek(p, ntiles, t, tile)) break;
+      if (tile.tn <= 0) continue;
       const int col0 = part * (tile.few ? 32 : L::kPartCols);   // this part's accumulator columns
       // the tokens of this warp's lanes' scales: its accumulator lanes, or where tokens are few its columns
       const int mine = tile.row0 + (tile.few ? col0 : (int)rank * 128 + quad * 32);
@@ -243,111 +341,103 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       float acc[L::kPartCols];
 #pragma unroll
       for (int i = 0; i < L::kPartCols; ++i) acc[i] = 0.0f;
-      // The scales of four K blocks are on their way while four are used: they come from L2, which under
-      // this load takes longer than a block.
-      float s_next[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s_next[i] = i < p.kblocks ? ld_ordered(sa_row + (size_t)i * p.pitch) * ld_ordered(sb_row + i) : 0.0f;
-      for (int kb0 = 0; kb0 < p.kblocks && ok; kb0 += 4) {
-        float s_now[4], sa[4], sb[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s_now[i] = s_next[i];
-          const int kb = min(kb0 + 4 + i, p.kblocks - 1);
-          sa[i] = ld_ordered(sa_row + (size_t)kb * p.pitch);
-          sb[i] = ld_ordered(sb_row + kb);
+      // One K block: waits for its accumulators, hands them back as soon as they are read.
+      auto block = [&](float s) {
+        if (!wait_accumulators(sbase + L::kBarAccFull + 8 * slot, parity, abort_flag)) {
+          ok = false;
+          return;
         }
+        tc_fence_after_sync();
+        const uint32_t tacc = tmem_base + lane_base + slot * 256 + col0;
+        const uint32_t empty = (sbase + L::kBarAccEmpty + 8 * slot) & kLeaderMask;
+        parity ^= slot;   // (two accumulators)
+        slot ^= 1u;
+        if (idle) {
+          tc_fence_before_sync();
+          if (lane == 0) mbar_arrive_cluster(empty);
+        } else if (tile.few) {
+          uint32_t d[32];
+          tmem_ld_32x32b_x32(tacc, d);
+          tmem_ld_wait();
+          tc_fence_before_sync();
+          if (lane == 0) mbar_arrive_cluster(empty);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (kb0 + i < p.kblocks && ok) {
-            ok = warp_wait(sbase + L::kBarAccFull + 8 * slot, parity, abort_flag, p.status, 4);
-            tc_fence_after_sync();
-            const uint32_t tacc = tmem_base + lane_base + slot * 256 + col0;
-            const uint32_t empty = (sbase + L::kBarAccEmpty + 8 * slot) & kLeaderMask;
-            if (++slot == L::kSlots) {
-              slot = 0;
-              parity ^= 1u;
+          for (int e = 0; e < 32; ++e) acc[e] = fmaf(__uint_as_float(d[e]), __shfl_sync(0xffffffffu, s, e), acc[e]);
+        } else {
+          // (no branches in here: the compiler then reads the next piece while it adds this one)
+#pragma unroll
+          const uint64_t s2 = pair_f32(s, s);
+#pragma unroll
+          for (int c = 0; c < L::kPartCols / 16; ++c) {
+            uint32_t d[16];
+            tmem_ld_32x32b_x16(tacc + c * 16, d);
+            tmem_ld_wait();
+            if (c == L::kPartCols / 16 - 1) {   // all read: the accumulator may be overwritten
+              tc_fence_before_sync();
+              if (lane == 0) mbar_arrive_cluster(empty);
             }
-            if (idle || !ok) {
-              tc_fence_before_sync();
-              if (lane == 0) mbar_arrive_cluster(empty);
-            } else if (tile.few) {
-              uint32_t d[32];
-              tmem_ld_32x32b_x32(tacc, d);
-              tmem_ld_wait();
-              tc_fence_before_sync();
-              if (lane == 0) mbar_arrive_cluster(empty);
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                acc[e] = fmaf(__uint_as_float(d[e]), __shfl_sync(0xffffffffu, s_now[i], e), acc[e]);
-            } else {
-              // (no branches in here: the compiler then reads the next piece while it adds this one)
-#pragma unroll
-              for (int c = 0; c < L::kPartCols / 32; ++c) {
-                uint32_t d[32];
-                tmem_ld_32x32b_x32(tacc + c * 32, d);
-                tmem_ld_wait();
-                if (c == L::kPartCols / 32 - 1) {   // all read: the accumulator may be overwritten
-                  tc_fence_before_sync();
-                  if (lane == 0) mbar_arrive_cluster(empty);
-                }
-#pragma unroll
-                for (int e = 0; e < 32; ++e) acc[c * 32 + e] = fmaf(__uint_as_float(d[e]), s_now[i], acc[c * 32 + e]);
-              }
+            for (int e = 0; e < 16; e += 2) {
+              float* a = acc + c * 16 + e;
+              const float2 sum = unpair_f32(fma_f32x2(pair_f32(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), s2, pair_f32(a[0], a[1])));
+              a[0] = sum.x;
+              a[1] = sum.y;
             }
           }
         }
+      };
+      // The scales of four K blocks are on their way while four are used: they come from L2, which under
+      // this load takes longer than a block.
+      const float* sa_at = sa_row + (size_t)kb_lo * p.pitch;
+      const float* sb_at = sb_row + kb_lo;
+      const size_t step = p.pitch;
+      int left = kb_hi - kb_lo;
+      float sa[4] = {}, sb[4] = {};
+      if (left >= 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_next[i] = sa[i] * sb[i];
-      }
-      if (!ok) break;
-
-      // ---- the sums leave, 32 columns at a time: turned around in the warp's box so that four lanes write
-      // 64 neighbouring bytes of a token
-      if (idle) continue;
-      const float rs = p.row_scale && mine + lane < p.rows_total ? ld_ordered(p.row_scale + mine + lane) : 1.0f;
-      const int first = tile.row0 + tile.lead, last = tile.row0 + tile.tn;
-      if (tile.few) {
-        // lanes are neighbouring columns of a token already
-        const int col = tile.nt * 256 + (int)rank * 128 + quad * 32 + lane;
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float v = acc[e] * __shfl_sync(0xffffffffu, rs, e);
-          const int row = mine + e;
-          if (row >= first && row < last && col < p.n) store_value(p, (size_t)row * p.n + col, v);
+        for (int i = 0; i < 4; ++i) {
+          sa[i] = ld_ordered(sa_at + i * step);
+          sb[i] = ld_ordered(sb_at + i);
         }
+      }
+      while (left >= 4 && ok) {
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] = sa[i] * sb[i];
+        sa_at += 4 * step;
+        sb_at += 4;
+        left -= 4;
+        if (left >= 4) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sa[i] = ld_ordered(sa_at + i * step);
+            sb[i] = ld_ordered(sb_at + i);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (ok) block(s[i]);
+      }
+#pragma unroll 1
+      for (; left > 0 && ok; --left, sa_at += step, ++sb_at) block(ld_ordered(sa_at) * ld_ordered(sb_at));
+      if (!ok) {
+        if (lane == 0) {
+          *abort_flag = 1u;
+          atomicCAS(p.status, 0, kStatusTimeout | 4);
+        }
+        break;
+      }
+      if (idle) continue;
+      if (p.splits > 1) {   // left in the ring's memory, [column][lane]: nothing is loaded there any more
+        const uint32_t sums = sbase + L::kOffRing + (uint32_t)(col0 * 128 + quad * 32 + lane) * 4;
+#pragma unroll
+        for (int i = 0; i < L::kPartCols; ++i)
+          if (i < 32 || !tile.few) st_shared_f32(sums + i * 512, acc[i]);
         continue;
       }
 #pragma unroll
-      for (int c = 0; c < L::kPartCols / 32; ++c) {
-        const int col = tile.nt * 256 + col0 + c * 32;
-        if (col >= p.n) break;
-        if (p.out_type == 1) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {   // 16 columns are 64 bytes
-            __syncwarp();                 // the box has been read
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float* v = acc + c * 32 + h * 16 + i * 4;
-              st_shared_v4(box + lane * L::kBoxPitch + i * 16, __float_as_uint(v[0] * rs), __float_as_uint(v[1] * rs),
-                           __float_as_uint(v[2] * rs), __float_as_uint(v[3] * rs));
-            }
-            __syncwarp();
-            store_box(p, box, mine, first, last, col + h * 16, 4, lane);
-          }
-        } else {
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t w[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = pack_16bit(acc[c * 32 + 8 * i + 2 * j] * rs, acc[c * 32 + 8 * i + 2 * j + 1] * rs, p.out_type);
-            st_shared_v4(box + lane * L::kBoxPitch + i * 16, w[0], w[1], w[2], w[3]);
-          }
-          __syncwarp();
-          store_box(p, box, mine, first, last, col, 2, lane);
-        }
-      }
+      for (int c = 0; c < L::kPartCols / 32; ++c)
+        if (c == 0 || !tile.few) store_piece(p, tile, acc + c * 32, part * (tile.few ? 1 : L::kPartCols / 32) + c, (int)rank, quad, lane, box);
     }
   } else if (warp == kProducerWarp) {
     // ------------------------------ producer (both CTAs) ------------------------
@@ -358,6 +448,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
     bool ok = true;
     for (int t = pair; ok; t += npairs) {
       if (!cur.seek(p, ntiles, t, tile)) break;
+      if (tile.tn <= 0) continue;
       // rows of this CTA: weights in boxes of 128 or 16, tokens in boxes of 128, 32 or 16
       const int wrows = tile.few ? 128 : tile.width >> 1;
       const int wrow = tile.g * p.n + tile.nt * 256 + (int)rank * wrows;
@@ -365,7 +456,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       const int tokens1 = tile.few ? tile.width >> 1 : (max(tile.tn - 128, 0) + 31) & ~31;
       const int tokens = leader ? tokens0 : tokens1, trow = tile.row0 + (int)rank * (tile.few ? tokens0 : 128);
       const uint32_t bytes = (uint32_t)(2 * wrows + tokens0 + tokens1) * 128u;
-      for (int kb = 0; kb < p.kblocks; ++kb) {
+      for (int kb = kb_lo; kb < kb_hi; ++kb) {
         ok = warp_wait(sbase + L::kBarEmpty + 8 * s, ((bits >> s) & 1u) ^ 1u, abort_flag, p.status, 1);
         if (!ok) break;
         bits ^= 1u << s;
@@ -403,32 +494,60 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
       const uint64_t tdesc0 = operand_desc_sw128(sbase + L::kOffRing + L::kW);
       for (int t = pair; ok; t += npairs) {
         if (!cur.seek(p, ntiles, t, tile)) break;
+        if (tile.tn <= 0) continue;
         const uint32_t idesc = kIdescBase | ((uint32_t)(tile.width >> 3) << 17);
-        for (int kb = 0; kb < p.kblocks; ++kb) {
-          ok = warp_wait(sbase + L::kBarFull + 8 * s, (bits >> s) & 1u, abort_flag, p.status, 3) &&
-               warp_wait(sbase + L::kBarAccEmpty + 8 * slot, parity, abort_flag, p.status, 2);
+        const uint64_t adesc0 = tile.few ? wdesc0 : tdesc0, bdesc0 = tile.few ? tdesc0 : wdesc0;
+        for (int kb = kb_lo; kb < kb_hi; ++kb) {
+          ok = warp_wait(sbase + L::kBarFull + 8 * s, (bits >> s) & 1u, abort_flag, p.status, 3);
           if (!ok) break;
           bits ^= 1u << s;
-          tc_fence_after_sync();
+          // all made ready before the wait: what lies between a free accumulator and the next product is on the
+          // critical path
           const uint32_t at = (uint32_t)s * ((uint32_t)stage_bytes >> 4);   // descriptors count 16-byte units
+          const uint64_t adesc = adesc0 + at, bdesc = bdesc0 + at;
+          const uint32_t acc = tmem_base + slot * 256, full = sbase + L::kBarAccFull + 8 * slot, empty = sbase + L::kBarEmpty + 8 * s;
+          ok = warp_wait(sbase + L::kBarAccEmpty + 8 * slot, parity, abort_flag, p.status, 2);
+          if (!ok) break;
+          tc_fence_after_sync();
           if (elect_one()) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              tc_mma_f8_pair(tmem_base + slot * 256, (tile.few ? wdesc0 : tdesc0) + at + 2 * j, (tile.few ? tdesc0 : wdesc0) + at + 2 * j, idesc, j > 0 ? 1u : 0u);
-            tc_commit_pair(sbase + L::kBarAccFull + 8 * slot, 3);
-            tc_commit_pair(sbase + L::kBarEmpty + 8 * s, 3);
+            for (int j = 0; j < 4; ++j) tc_mma_f8_pair(acc, adesc + 2 * j, bdesc + 2 * j, idesc, j > 0 ? 1u : 0u);
+            tc_commit_pair(full, both);
+            tc_commit_pair(empty, both);
           }
           __syncwarp();
           s = (s + 1 == stages) ? 0 : s + 1;
-          if (++slot == L::kSlots) {
-            slot = 0;
-            parity ^= 1u;
-          }
+          parity ^= slot;   // (two accumulators)
+          slot ^= 1u;
         }
       }
     }
   }
 
+  if (p.splits > 1) {
+    cluster_sync();   // every pair's sums are in place
+    Fp8Cursor cur;
+    Fp8Tile tile;
+    if (warp < L::kEpiWarps && cur.seek(p, ntiles, pair, tile) && tile.tn > 0) {
+      const int quad = warp & 3;
+      const uint32_t box = sbase + L::kOffBox + warp * L::kBoxBytes;
+      const int pieces = tile.width >> 5;
+      // lanes without a token are left out like the pairs' own warps left them out
+      const bool there = tile.few || (int)rank * 128 + quad * 32 < tile.tn;
+      for (int pc = share + p.splits * (warp >> 2); pc < pieces && there; pc += 2 * p.splits) {
+        float v[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+        for (int s = 0; s < p.splits; ++s) {
+          const uint32_t from = cluster_map_shared(sbase + L::kOffRing + (uint32_t)(pc * 4096 + quad * 32 + lane) * 4, 2 * s + rank);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) v[e] += ld_shared_cluster_f32(from + e * 512);
+        }
+        store_piece(p, tile, v, pc, (int)rank, quad, lane, box);
+      }
+    }
+    __syncwarp();
+  }
   tc_fence_before_sync();
   __syncthreads();
   if (*abort_flag) {
@@ -483,12 +602,33 @@ static int gemm_fp8_block(const void* a_q, const float* a_sf, const void* b_q, c
   p.kblocks = (k + 127) / 128; p.nblocks = (n + 127) / 128;
   const int sms = num_sms();
   if (sms <= 0) return fail(MSC_ERR_CUDA, "could not query the SM count");
-  int pairs = (max_ctas > 0 && max_ctas < sms ? max_ctas : sms) / 2;
-  if (pairs < 1) pairs = 1;
-  if (pairs > max_tiles) pairs = (int)max_tiles;
+  const int ctas = max_ctas > 0 && max_ctas < sms ? max_ctas : sms;
+  const int room = ctas >= 2 ? ctas / 2 : 1;   // CTA pairs
+  p.splits = 1;
+  p.quarters_from = 0x7fffffff;
+  long long units = max_tiles;                 // tiles, or clusters' pairs
+  if (!group_rows) {
+    const long long tiles = ((long long)rows_total + 255) / 256 * ntiles;
+    const int rest = rows_total % 256;
+    const long long whole = rest >= 1 && rest <= Fp8Smem::kFewTokens ? tiles - ntiles : tiles;   // more than 64 tokens
+    const long long done = tiles / room * room;
+    units = tiles;
+    while (p.splits < 4 && tiles * p.splits * 2 <= room && p.kblocks >= 8 * p.splits) p.splits *= 2;
+    if (p.splits > 1) {
+      units = tiles * p.splits;
+    } else if (whole > done && 4 * (whole - done) + (tiles - whole) <= room) {
+      p.quarters_from = (int)done;
+      units = done + 4 * (tiles - done);
+    }
+  }
+  const int pairs = (int)(units < room ? units : room);
   if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(gemm_fp8_block_kernel), Fp8Smem::kAlloc)) return rc;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t lc = pdl_launch_config(2 * pairs, Fp8Smem::kThreads, Fp8Smem::kAlloc, static_cast<cudaStream_t>(stream), attr);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2u * (unsigned)p.splits;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1u;
+  lc.numAttrs = 2;
   MSC_CUDA_OK(cudaLaunchKernelEx(&lc, gemm_fp8_block_kernel, tw, tw16, t128, t32, t16, p));
   return MSC_OK;
 }

@@ -225,6 +225,21 @@ def test_dense(m, n, k, exact):
     _check(few, want, mags, k, "f32", exact)
 
 
+@pytest.mark.parametrize("m,n,k,ctas", [(1792, 256, 272, 12), (1797, 256, 1040, 12), (1700, 256, 128, 12), (256, 264, 400, 16), (520, 1000, 272, 28),
+                                        (100, 1304, 640, 0), (4101, 520, 272, 0)])
+def test_last_round_in_quarter_tiles(m, n, k, ctas):
+    """Grids whose last round of tiles would be nearly empty: those tiles are taken in quarters, some of which are empty."""
+    from mosaicist_b200 import ops
+
+    rng = np.random.default_rng([m, n, k])
+    a, sa, b, sb = _operands(rng, m, 1, n, k, True)
+    want = F.product(a, sa, b[0], sb[0])[0]
+    out = torch.full((m + 9, n), 3.0, dtype=torch.float32, device="cuda")
+    got = ops.gemm_fp8_block(T(a), _dev_sf(sa), T(b[0]), T(sb[0]), out=out[:m], max_ctas=ctas)
+    _check(got, want, None, k, "f32", True)
+    assert (out[m:] == 3).all()
+
+
 def test_dense_writes_its_rows_only():
     from mosaicist_b200 import ops
 
