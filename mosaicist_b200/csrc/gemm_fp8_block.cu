@@ -365,7 +365,6 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
           for (int e = 0; e < 32; ++e) acc[e] = fmaf(__uint_as_float(d[e]), __shfl_sync(0xffffffffu, s, e), acc[e]);
         } else {
           // (no branches in here: the compiler then reads the next piece while it adds this one)
-#pragma unroll
           const uint64_t s2 = pair_f32(s, s);
 #pragma unroll
           for (int c = 0; c < L::kPartCols / 16; ++c) {

@@ -36,6 +36,7 @@ struct RouteParams {
   int tokens, experts, topk;
   int groups, topk_groups, group_top;   // groups = 1: no restriction
   int per, slots;        // experts and register slots of a group
+  int base[32];          // lane 0's expert of every slot
   int renormalize;
   int by_score;          // keys are scores (+ bias), else logits
   float scale;
@@ -62,10 +63,15 @@ __device__ __forceinline__ float warp_max(float v) {
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
+// In the order of their bits (negative ones turned round), high words first: two reductions instead of five
+// rounds of shuffles.  (-0 comes out below +0, which no comparison tells apart.)
 __device__ __forceinline__ double warp_max(double v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+  const long long bits = __double_as_longlong(v);
+  const unsigned long long o = (unsigned long long)bits ^ ((unsigned long long)(bits >> 63) | 0x8000000000000000ull);
+  const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(o >> 32));
+  const unsigned lo = __reduce_max_sync(0xffffffffu, (unsigned)(o >> 32) == hi ? (unsigned)o : 0u);
+  const unsigned long long m = (unsigned long long)hi << 32 | lo;
+  return __longlong_as_double((long long)(m ^ ((m >> 63) ? 0x8000000000000000ull : 0xffffffffffffffffull)));
 }
 // Every lane gets the same bits: the order of the additions is fixed.
 template <class F>
@@ -85,7 +91,12 @@ __device__ __forceinline__ float exp_fast(float x) {
 // e^(x - mx) where mx is the largest x: an infinite maximum leaves only the logits that equal it.
 __device__ __forceinline__ float exp_below(float x, float mx) { return x == mx ? (x == -INFINITY ? 0.0f : 1.0f) : exp_fast(x - mx); }
 __device__ __forceinline__ double exp_below(double x, double mx) { return x == mx ? (x == -INFINITY ? 0.0 : 1.0) : exp(x - mx); }
-__device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + exp_fast(-x)); }
+__device__ __forceinline__ float rcp_fast(float x) {   // one ulp
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float sigmoid(float x) { return rcp_fast(1.0f + exp_fast(-x)); }
 __device__ __forceinline__ double sigmoid(double x) { return 1.0 / (1.0 + exp(-x)); }
 
 // What lane `k` is handed by the choice of the k-th expert.
@@ -94,74 +105,82 @@ struct Pick {
   bool barred = true;
 };
 
-// Chooses from key[slot] of every lane.  `open`: bit per slot that holds an expert; base[slot]: its
-// lane 0's expert.  CHECK: returns whether two keys that the choice tells apart are closer than `tol`.
-template <int PER, class F, bool CHECK>
-__device__ __forceinline__ bool choose(const RouteParams& p, F (&key)[PER], F tol, uint32_t open, const int* base, int lane,
-                                       Pick& pick) {
+// The groups that take part, a bit each.  `near`: whether the last that does and the first that does not are
+// closer than `tol` (infinite differences of equal infinities come out NaN and count as near).
+template <int PER, class F>
+__device__ __forceinline__ uint32_t choose_groups(const RouteParams& p, const F (&key)[PER], F tol, int lane, bool& near) {
   const F kNone = -INFINITY;
-  bool near = false;
-  if (p.groups > 1) {
-    F strength = kNone;              // of group `lane`
+  F strength = kNone;              // of group `lane`
+  auto judge = [&](int g, F best, F second) {   // from every lane's best two keys of group g
+    F sum = warp_max(best);
+    if (p.group_top == 2) {
+      const int owner = __ffs(__ballot_sync(0xffffffffu, best == sum)) - 1;
+      const F next = warp_max(lane == owner ? second : best);
+      sum = (sum == kNone || next == kNone) ? kNone : sum + next;
+    }
+    if (lane == g) strength = sum;
+  };
+  if (p.slots == 1) {              // warp-uniform, as all of this
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (i < p.groups) judge(i, key[i], kNone);
+  } else {
     F best = kNone, second = kNone;
     int j = 0, g = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if (g < p.groups) {            // warp-uniform, as all of this
-        if (key[i] > best) {
-          second = best;
-          best = key[i];
-        } else if (key[i] > second) {
-          second = key[i];
-        }
-        if (++j == p.slots) {
-          F sum = warp_max(best);
-          if (p.group_top == 2) {
-            const int owner = __ffs(__ballot_sync(0xffffffffu, best == sum)) - 1;
-            const F next = warp_max(lane == owner ? second : best);
-            sum = (sum == kNone || next == kNone) ? kNone : sum + next;
-          }
-          if (lane == g) strength = sum;
-          best = second = kNone;
-          j = 0;
-          ++g;
-        }
+      if (key[i] > best) {
+        second = best;
+        best = key[i];
+      } else if (key[i] > second) {
+        second = key[i];
       }
-    }
-    int ahead = 0;
-    for (int o = 0; o < p.groups; ++o) {
-      const F other = __shfl_sync(0xffffffffu, strength, o);
-      ahead += (other > strength || (other == strength && o < lane)) ? 1 : 0;
-    }
-    const bool kept = lane < p.groups && ahead < p.topk_groups;
-    const uint32_t in = __ballot_sync(0xffffffffu, kept);
-    if (CHECK) {
-      const F weakest = -warp_max(kept ? -strength : kNone);
-      const F left = warp_max(lane < p.groups && !kept ? strength : kNone);
-      // (infinite differences of equal infinities come out NaN and count as near)
-      near = left != kNone && !(weakest - left > tol * (F)p.group_top);
-    }
-    j = g = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (!((in >> g) & 1u)) key[i] = kNone;
       if (++j == p.slots) {
+        if (g < p.groups) judge(g, best, second);
+        best = second = kNone;
         j = 0;
-        g = min(g + 1, 31);
+        ++g;
       }
     }
   }
-  F before = kNone;
-  for (int k = 0; k < p.topk + (CHECK ? 1 : 0); ++k) {
+  int ahead = 0;
+  for (int o = 0; o < p.groups; ++o) {
+    const F other = __shfl_sync(0xffffffffu, strength, o);
+    ahead += (other > strength || (other == strength && o < lane)) ? 1 : 0;
+  }
+  const bool kept = lane < p.groups && ahead < p.topk_groups;
+  const F weakest = -warp_max(kept ? -strength : kNone);
+  const F left = warp_max(lane < p.groups && !kept ? strength : kNone);
+  near = left != kNone && !(weakest - left > tol * (F)p.group_top);
+  return __ballot_sync(0xffffffffu, kept);
+}
+
+template <int PER, class F>
+__device__ __forceinline__ void bar_groups(const RouteParams& p, F (&key)[PER], uint32_t in) {
+  int j = 0, g = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (!((in >> g) & 1u)) key[i] = -INFINITY;
+    if (++j == p.slots) {
+      j = 0;
+      g = min(g + 1, 31);
+    }
+  }
+}
+
+// Chooses from key[slot] of every lane, whatever the keys.  `open`: bit per slot that holds an expert;
+// base[slot]: its lane 0's expert.
+template <int PER, class F>
+__device__ __forceinline__ void choose_any(const RouteParams& p, F (&key)[PER], uint32_t open, const int* base, int lane, Pick& pick) {
+  if (p.groups > 1) {
+    bool near;
+    bar_groups(p, key, choose_groups<PER, F>(p, key, (F)0, lane, near));
+  }
+  for (int k = 0; k < p.topk; ++k) {
     F m = key[0];
 #pragma unroll
     for (int i = 1; i < PER; ++i) m = key[i] > m ? key[i] : m;
     m = warp_max(m);
-    if (CHECK) {
-      if (k > 0 && m != kNone && !(before - m > tol)) near = true;
-      if (k == p.topk) break;
-      before = m;
-    }
     int slot = -1;
 #pragma unroll
     for (int i = PER - 1; i >= 0; --i)
@@ -172,14 +191,76 @@ __device__ __forceinline__ bool choose(const RouteParams& p, F (&key)[PER], F to
       open &= ~(1u << slot);
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        if (i == slot) key[i] = kNone;
+        if (i == slot) key[i] = -INFINITY;
     }
     if (lane == k) {
       pick.id = won;
-      pick.barred = m == kNone;
+      pick.barred = m == (F)-INFINITY;
     }
   }
-  return near;
+}
+
+// The same at a quarter of the instructions, for the usual case.  Every lane keeps its two best keys at hand and looks
+// through its slots again only when both are gone (a lane that holds three of the best).  Returns false where
+// the choice has to be made over again: two keys that it tells apart are closer than `tol` (CHECK), or
+// fewer than topk experts are left.
+template <int PER, bool CHECK>
+__device__ __forceinline__ bool choose(const RouteParams& p, float (&key)[PER], float tol, const int* base, int lane, Pick& pick) {
+  const float kNone = -INFINITY;
+  if (p.groups > 1) {
+    bool near;
+    const uint32_t in = choose_groups<PER, float>(p, key, tol, lane, near);
+    if (CHECK && near) return false;
+    bar_groups(p, key, in);
+  }
+  float best, second;
+  int best_at, second_at, best_id, second_id;
+  uint32_t taken = 0;              // slots
+  auto look = [&] {
+    best = second = kNone;
+    best_at = second_at = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const float v = (taken >> i) & 1u ? kNone : key[i];
+      if (v > second) {
+        const bool top = v > best;
+        second = top ? best : v;
+        second_at = top ? best_at : i;
+        best = top ? v : best;
+        best_at = top ? i : best_at;
+      }
+    }
+    best_id = base[best_at] + lane;
+    second_id = base[second_at] + lane;
+  };
+  look();
+  bool fine = true;
+  float before = INFINITY;
+  for (int k = 0; k < p.topk; ++k) {
+    const float m = warp_max(best);
+    fine = fine && m != kNone;
+    if (CHECK) {
+      fine = fine && (k == 0 || before - m > tol);
+      before = m;
+    }
+    const int mine = best == m ? best_id : 0x7fffffff;
+    const int won = __reduce_min_sync(0xffffffffu, mine);
+    if (mine == won) {
+      taken |= 1u << best_at;
+      best = second;
+      best_at = second_at;
+      best_id = second_id;
+      second = kNone;
+      if (best == kNone) look();
+    }
+    if (lane == k) pick.id = won;
+  }
+  if (CHECK) {                     // the best that is left
+    const float m = warp_max(best);
+    fine = fine && (m == kNone || before - m > tol);
+  }
+  pick.barred = false;
+  return fine;
 }
 
 // The choice of a token in 64 bits.
@@ -192,28 +273,30 @@ __device__ __noinline__ Pick choose_in_64_bits(const RouteParams& p, const T* ro
     key[i] = ((open >> i) & 1u) ? (double)load_logit(row + base[i] + lane) : -INFINITY;
     mx = fmax(mx, key[i]);
   }
-  if (!SIGMOID) {
-    mx = warp_max(mx);
+  if (p.by_score) {
+    if (!SIGMOID) {
+      mx = warp_max(mx);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sum += exp_below(key[i], mx);
-    sum = warp_sum(sum);
-  }
+      for (int i = 0; i < PER; ++i) sum += exp_below(key[i], mx);
+      sum = warp_sum(sum);
+    }
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const double x = key[i];
-    const double b = (p.bias && ((open >> i) & 1u)) ? (double)ld_ordered(p.bias + base[i] + lane) : 0.0;
-    const double s = SIGMOID ? sigmoid(x) : sum > 0.0 ? exp_below(x, mx) / sum : 0.0;
-    key[i] = (x == -INFINITY || b != b) ? -INFINITY : s + b;
+    for (int i = 0; i < PER; ++i) {
+      const double x = key[i];
+      const double b = (p.bias && ((open >> i) & 1u)) ? (double)ld_ordered(p.bias + base[i] + lane) : 0.0;
+      const double s = SIGMOID ? sigmoid(x) : sum > 0.0 ? exp_below(x, mx) / sum : 0.0;
+      key[i] = (x == -INFINITY || b != b) ? -INFINITY : s + b;
+    }
   }
   Pick pick;
-  choose<PER, double, false>(p, key, 0.0, open, base, lane, pick);
+  choose_any<PER, double>(p, key, open, base, lane, pick);
   return pick;
 }
 
 template <int PER, bool SIGMOID, class T>
 __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
   __shared__ int base[32];
-  if (threadIdx.x < 32) base[threadIdx.x] = (int)(threadIdx.x / p.slots) * p.per + (int)(threadIdx.x % p.slots) * 32;
+  if (threadIdx.x < 32) base[threadIdx.x] = p.base[threadIdx.x];
   __syncthreads();
   grid_dependency_wait();
   grid_launch_dependents();
@@ -222,7 +305,7 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
   if (token >= p.tokens) return;
   const T* row = static_cast<const T*>(p.logits) + token * p.experts;
 
-  float key[PER];
+  float key[PER], b[PER];
   uint32_t open = 0;
   {
     int j = 0, g = 0;
@@ -230,6 +313,7 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
     for (int i = 0; i < PER; ++i) {
       if (g < p.groups && j * 32 + lane < p.per) open |= 1u << i;
       key[i] = ((open >> i) & 1u) ? load_logit(row + base[i] + lane) : -INFINITY;
+      b[i] = (p.bias && ((open >> i) & 1u)) ? ld_ordered(p.bias + base[i] + lane) : 0.0f;
       if (++j == p.slots) {
         j = 0;
         ++g;
@@ -246,27 +330,28 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
     sum = warp_sum(sum);
   }
   Pick pick;
+  bool fine;
   if (p.by_score) {
     const float inv = sum > 0.0f ? __fdividef(1.0f, sum) : 0.0f;
     float largest = 0.0f;   // magnitude of a key
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const float x = key[i];
-      const float b = (p.bias && ((open >> i) & 1u)) ? ld_ordered(p.bias + base[i] + lane) : 0.0f;
       const float s = SIGMOID ? sigmoid(x) : exp_below(x, mx) * inv;
-      key[i] = (x == -INFINITY || b != b) ? -INFINITY : s + b;
-      if (key[i] != -INFINITY) largest = fmaxf(largest, fabsf(key[i]));
+      const float v = s + b[i];
+      key[i] = (x == -INFINITY || v != v) ? -INFINITY : v;   // (a NaN is the bias')
+      largest = fmaxf(largest, key[i] == -INFINITY ? 0.0f : fabsf(key[i]));
     }
     // What a key may be off by, twice.  Sigmoid: s (1 - s) (|x| 2^-24 + 2^-22) from the exponential, at
     // most 1.4e-7, the sum and the quotient 3 x 2^-24 s.  Softmax: 2^-22 + |x - max| 2^-24 of p from its
     // exponential (p |x - max| is at most 1/e of the largest p, which is `inv`), as much and up to 37
     // additions' 2^-24 from the sum, and the quotient: 51 x 2^-24.  Then the rounding of the key itself.
     const float tol = (SIGMOID ? 0x1p-20f : 0x1p-17f * inv) + 0x1p-22f * warp_max(largest);
-    if (choose<PER, float, true>(p, key, tol, open, base, lane, pick))
-      pick = choose_in_64_bits<PER, SIGMOID, T>(p, row, open, base, lane);
+    fine = choose<PER, true>(p, key, tol, base, lane, pick);
   } else {
-    choose<PER, float, false>(p, key, 0.0f, open, base, lane, pick);
+    fine = choose<PER, false>(p, key, 0.0f, base, lane, pick);
   }
+  if (!fine) pick = choose_in_64_bits<PER, SIGMOID, T>(p, row, open, base, lane);
 
   // the weights, lane k that of the k-th choice, from the logits again
   const bool there = lane < p.topk && !pick.barred;
@@ -437,6 +522,7 @@ int msc_moe_route(const void* logits, int dtype, const float* bias, int32_t* ids
   if (p.groups * p.slots > 32)
     return fail(MSC_ERR_UNSUPPORTED, "%d groups of %d experts: groups x (experts of a group / 32, rounded up) must be at most 32",
                 groups, per);
+  for (int i = 0; i < 32; ++i) p.base[i] = i / p.slots * p.per + i % p.slots * 32;
   p.renormalize = cfg->renormalize != 0;
   p.by_score = bias != nullptr || (limited && cfg->group_top == 2);
   p.scale = cfg->scale;
