@@ -14,6 +14,8 @@
 
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 namespace msc {
 
 constexpr float kFp8Max = 448.0f;
@@ -62,6 +64,12 @@ template <> struct Vec16<__nv_bfloat16> {
       v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
+  // largest magnitude, NaNs left out; two values an instruction
+  static __device__ __forceinline__ float amax(const uint4& r) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+    const float2 f = __bfloat1622float2(__hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3]))));
+    return fmaxf(fmaxf(0.0f, f.x), f.y);
+  }
 };
 template <> struct Vec16<__half> {
   static constexpr int kPer = 8;
@@ -74,6 +82,11 @@ template <> struct Vec16<__half> {
       v[2 * i + 1] = f.y;
     }
   }
+  static __device__ __forceinline__ float amax(const uint4& r) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    const float2 f = __half22float2(__hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3]))));
+    return fmaxf(fmaxf(0.0f, f.x), f.y);
+  }
 };
 template <> struct Vec16<float> {
   static constexpr int kPer = 4;
@@ -81,18 +94,11 @@ template <> struct Vec16<float> {
     v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y);
     v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
   }
+  static __device__ __forceinline__ float amax(const uint4& r) {
+    return fmaxf(fmaxf(fabsf(__uint_as_float(r.x)), fabsf(__uint_as_float(r.y))),
+                 fmaxf(fmaxf(0.0f, fabsf(__uint_as_float(r.z))), fabsf(__uint_as_float(r.w))));
+  }
 };
-
-// 16 consecutive values (16-byte aligned).
-template <class T>
-__device__ __forceinline__ void load_16(const T* src, float* v) {
-  constexpr int kVecs = 16 / Vec16<T>::kPer;
-  uint4 raw[kVecs];
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) raw[i] = ld_ordered(reinterpret_cast<const uint4*>(src) + i);
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) Vec16<T>::unpack(raw[i], v + i * Vec16<T>::kPer);
-}
 
 struct RowBlockParams {
   const void* x;             // (rows, k), with SILU (rows, 2k) gate | up
@@ -104,17 +110,18 @@ struct RowBlockParams {
 };
 
 // ---- activations ---------------------------------------------------------------------------
-// A CTA takes 8 rows x 512 columns, a warp one of the rows, a thread 16 values: 8 lanes share a block.  The
-// 32 scales of the tile meet in shared memory and leave as 32-byte pieces of the column layout.
+// A CTA takes 8 rows, a warp one of them, and walks its share of the row's pieces of 512 columns with the next
+// piece's loads in flight; a thread holds 16 values, 8 lanes share a block.  The 32 scales of a
+// piece meet in shared memory and leave as 32-byte stretches of the column layout.
 template <class T, bool SILU>
 __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const RowBlockParams p) {
   grid_dependency_wait();
   grid_launch_dependents();
-  __shared__ float s_scale[8][4];
+  __shared__ float s_scale[2][8][4];
   __shared__ unsigned s_live;
+  constexpr int kVecs = 16 / Vec16<T>::kPer;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row0 = blockIdx.y * 8, row = row0 + warp;
-  const int col = blockIdx.x * 512 + lane * 16;
 
   // the rows of the tile that take part: all of them, or those that some group owns
   unsigned live = row0 + 8 <= p.rows ? 0xffu : (1u << max(p.rows - row0, 0)) - 1u;
@@ -129,35 +136,51 @@ __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const RowBlockPa
     __syncthreads();
     live &= s_live;
   }
-  if (live || row0 + 8 > p.rows) {   // (the last rows' tile also clears the scale columns behind them)
-    const bool mine = ((live >> warp) & 1u) && col < p.k;
-    float v[16];
+  if (live == 0 && row0 + 8 <= p.rows) return;   // (the last rows' tile also clears the scale columns behind them)
+  const bool mine = (live >> warp) & 1u;
+  const T* src = static_cast<const T*>(p.x) + (size_t)row * p.k * (SILU ? 2 : 1) + lane * 16;
+  uint4 raw[kVecs * (SILU ? 2 : 1)];
+  auto load = [&](int c) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-    if (mine) {
-      if (SILU) {
-        const T* src = static_cast<const T*>(p.x) + (size_t)row * 2 * p.k + col;
-        float up[16];
-        load_16(src, v);
-        load_16(src + p.k, up);
+    for (int i = 0; i < kVecs * (SILU ? 2 : 1); ++i) raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (mine && c * 512 + lane * 16 < p.k) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = silu_mul(v[i], up[i]);
-      } else {
-        load_16(static_cast<const T*>(p.x) + (size_t)row * p.k + col, v);
+      for (int i = 0; i < kVecs; ++i) {
+        raw[i] = ld_ordered(reinterpret_cast<const uint4*>(src + c * 512) + i);
+        if (SILU) raw[kVecs * (SILU ? 1 : 0) + i] = ld_ordered(reinterpret_cast<const uint4*>(src + p.k + c * 512) + i);
       }
     }
-    float amax = amax_f32x16(v);
+  };
+  const int pieces = (p.k + 511) >> 9;
+  load(blockIdx.x);
+  for (int c = blockIdx.x, buf = 0; c < pieces; c += gridDim.x, buf ^= 1) {
+    float v[16], amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      if (!SILU) amax = fmaxf(amax, Vec16<T>::amax(raw[i]));
+      Vec16<T>::unpack(raw[i], v + i * Vec16<T>::kPer);
+    }
+    if (SILU) {
+      float up[16];
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) Vec16<T>::unpack(raw[kVecs * (SILU ? 1 : 0) + i], up + i * Vec16<T>::kPer);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = silu_mul(v[i], up[i]);
+      amax = amax_f32x16(v);
+    }
+    if (c + (int)gridDim.x < pieces) load(c + gridDim.x);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     const float s = block_scale(amax);
-    if ((lane & 7) == 0) s_scale[warp][lane >> 3] = s;
-    if (mine) *reinterpret_cast<uint4*>(p.q + (size_t)row * p.k + col) = pack_e4m3_16(v, s);
+    if ((lane & 7) == 0) s_scale[buf][warp][lane >> 3] = s;
+    const int col = c * 512 + lane * 16;
+    if (mine && col < p.k) *reinterpret_cast<uint4*>(p.q + (size_t)row * p.k + col) = pack_e4m3_16(v, s);
     __syncthreads();
     if (threadIdx.x < 32) {
-      const int c = blockIdx.x * 4 + (threadIdx.x >> 3), r = threadIdx.x & 7;
-      if (c < p.kblocks) {
-        if ((live >> r) & 1u) p.sf[(size_t)c * p.pitch + row0 + r] = s_scale[r][threadIdx.x >> 3];
-        else if (row0 + r >= p.rows && row0 + r < p.pitch) p.sf[(size_t)c * p.pitch + row0 + r] = 0.0f;
+      const int kb = c * 4 + (threadIdx.x >> 3), r = threadIdx.x & 7;
+      if (kb < p.kblocks) {
+        if ((live >> r) & 1u) p.sf[(size_t)kb * p.pitch + row0 + r] = s_scale[buf][r][threadIdx.x >> 3];
+        else if (row0 + r >= p.rows && row0 + r < p.pitch) p.sf[(size_t)kb * p.pitch + row0 + r] = 0.0f;
       }
     }
   }
@@ -174,7 +197,7 @@ struct WeightBlockParams {
 };
 
 template <class T>
-__global__ void __launch_bounds__(256) quantize_fp8_weight_kernel(const WeightBlockParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 2 : 4) quantize_fp8_weight_kernel(const WeightBlockParams p) {
   __shared__ float s_amax[8];
   constexpr int kVecs = 16 / Vec16<T>::kPer;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -192,11 +215,9 @@ __global__ void __launch_bounds__(256) quantize_fp8_weight_kernel(const WeightBl
   float amax = 0.0f;
   float v[16];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < kVecs; ++j) Vec16<T>::unpack(raw[i][j], v + j * Vec16<T>::kPer);
-    amax = fmaxf(amax, amax_f32x16(v));
-  }
+    for (int j = 0; j < kVecs; ++j) amax = fmaxf(amax, Vec16<T>::amax(raw[i][j]));
 #pragma unroll
   for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (lane == 0) s_amax[warp] = amax;
@@ -216,9 +237,14 @@ __global__ void __launch_bounds__(256) quantize_fp8_weight_kernel(const WeightBl
 
 template <class T>
 static int launch_rows(const RowBlockParams& p, bool silu, cudaStream_t stream) {
+  const int sms = num_sms();
+  if (sms <= 0) return fail(MSC_ERR_CUDA, "could not query the SM count");
+  // as many CTAs per row as it takes to give every SM sixteen
+  const int tiles = (p.rows + 7) / 8, pieces = (p.k + 511) / 512;
+  const int split = std::max(1, std::min(pieces, (16 * sms + tiles - 1) / tiles));
   cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t lc = pdl_launch_config((p.k + 511) / 512, 256, 0, stream, attr);
-  lc.gridDim.y = (unsigned)((p.rows + 7) / 8);
+  cudaLaunchConfig_t lc = pdl_launch_config(split, 256, 0, stream, attr);
+  lc.gridDim.y = (unsigned)tiles;
   auto kern = silu ? quantize_fp8_rows_kernel<T, true> : quantize_fp8_rows_kernel<T, false>;
   MSC_CUDA_OK(cudaLaunchKernelEx(&lc, kern, p));
   return MSC_OK;
