@@ -300,6 +300,16 @@ int msc_grouped_gemm_bf16_int4_ragged(const void* a, const void* b_q, const void
 int msc_fp8_block_quantize(const void* x, int x_dtype, int silu, const int32_t* group_offsets,
                            const int32_t* group_rows, void* q, float* sf, int l, int rows, int k, void* stream);
 
+/* The dispatch of the routed layer in this format: gathers each locally routed token row (tokens (tokens,
+ * hidden) bf16), quantises it once and writes it at row group_offsets[e] + rank (msc_moe_plan) of a_q (rows_cap,
+ * hidden) and a_sf (ceil(hidden / 128), rows_cap rounded up to 4), with the pair's routing weight in row_weight
+ * (rows_cap) f32 and its token in row_token (rows_cap) i32.  hidden % 16 == 0, topk <= 64, a_q 16-byte
+ * aligned; a row that would lie at or beyond rows_cap is left out.  tokens = 0 does nothing. */
+int msc_moe_permute_quantize_fp8_block(const void* tokens_bf16, const int32_t* ids, const float* weights,
+                                       const int32_t* rank, const int32_t* group_offsets, int tokens, int hidden,
+                                       int topk, int expert_first, int experts_local, void* a_q, float* a_sf,
+                                       float* row_weight, int32_t* row_token, int rows_cap, void* stream);
+
 /* w (l, n, k) -> q (l, n, k) bytes, sf (l, ceil(n / 128), ceil(k / 128)) f32. */
 int msc_fp8_block_quantize_weight(const void* w, int w_dtype, void* q, float* sf, int l, int n, int k,
                                   void* stream);

@@ -72,6 +72,7 @@ SIGNATURES = {
     "msc_moe_route_backward": (_I, [_P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_float, _P]),
     "msc_fp8_block_quantize": (_I, [_P, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P]),
     "msc_fp8_block_quantize_weight": (_I, [_P, _I, _P, _P, _I, _I, _I, _P]),
+    "msc_moe_permute_quantize_fp8_block": (_I, [_P] * 5 + [_I] * 5 + [_P] * 4 + [_I, _P]),
     "msc_gemm_fp8_block": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "msc_grouped_gemm_fp8_block_ragged": (_I, [_P] * 8 + [_I] * 6 + [_P]),
     "msc_moe_plan": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _P]),

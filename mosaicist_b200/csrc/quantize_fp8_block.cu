@@ -186,6 +186,80 @@ __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const RowBlockPa
   }
 }
 
+// ---- dispatch of the routed layer ------------------------------------------------------------
+// CTAs walk the tokens; a token's row is quantised once into shared memory and leaves for the row of every
+// expert it is routed to as one bulk copy, the scales as words of their column layout.  Two row buffers
+// alternate, so the copies of one token leave while the next is quantised.
+struct Fp8DispatchParams {
+  const __nv_bfloat16* tokens;   // (tokens, hidden)
+  const int* ids;                // (tokens, topk)
+  const float* weights;          // (tokens, topk)
+  const int* rank;               // (tokens, topk)
+  const int* group_offsets;      // (experts_local)
+  uint8_t* q;                    // (rows_cap, hidden)
+  float* sf;                     // (kblocks, pitch)
+  float* row_weight;             // (rows_cap)
+  int* row_token;                // (rows_cap)
+  int hidden, kblocks, topk, expert_first, experts_local, rows_cap, pitch;
+};
+
+constexpr int kFp8MaxTopk = 64;
+
+__global__ void __launch_bounds__(512) moe_permute_quantize_fp8_kernel(const Fp8DispatchParams p, int tokens) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  extern __shared__ __align__(16) uint8_t row_smem[];   // 2 x ([hidden] values, [kblocks] scales)
+  __shared__ int s_dest[2][kFp8MaxTopk];
+  const int row_bytes = (p.hidden + 4 * p.kblocks + 15) & ~15;
+  const int padded = (p.hidden + 127) & ~127;           // the eight lanes of a block stay together
+  int it = 0;
+  for (long long token = blockIdx.x; token < tokens; token += gridDim.x, ++it) {
+    const int buf = it & 1;
+    uint8_t* s_q = row_smem + buf * row_bytes;
+    float* s_sf = reinterpret_cast<float*>(s_q + p.hidden);
+    // the copies of the token before last have read this buffer; the last token's may still run
+    if (threadIdx.x == 0) bulk_wait_group_read1();
+    if ((int)threadIdx.x < p.topk) {
+      const long long pair = token * p.topk + threadIdx.x;
+      const int e = ld_ordered(p.ids + pair) - p.expert_first;
+      int dest = -1;
+      if (e >= 0 && e < p.experts_local) {
+        dest = ld_ordered(p.group_offsets + e) + ld_ordered(p.rank + pair);
+        if (dest < 0 || dest >= p.rows_cap) {
+          dest = -1;
+        } else {
+          p.row_weight[dest] = ld_ordered(p.weights + pair);
+          p.row_token[dest] = (int)token;
+        }
+      }
+      s_dest[buf][threadIdx.x] = dest;
+    }
+    __syncthreads();
+    for (int col = threadIdx.x * 16; col < padded; col += blockDim.x * 16) {
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+      if (col < p.hidden) load16_bf16(p.tokens + (size_t)token * p.hidden + col, v);
+      float amax = amax_f32x16(v);
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffu << (threadIdx.x & 24u), amax, o));
+      const float s = block_scale(amax);
+      if (col < p.hidden) *reinterpret_cast<uint4*>(s_q + col) = pack_e4m3_16(v, s);
+      if ((threadIdx.x & 7) == 0) s_sf[col >> 7] = s;
+    }
+    fence_proxy_async_smem();
+    __syncthreads();
+    for (int k = 0; k < p.topk; ++k) {
+      const int dest = s_dest[buf][k];
+      if (dest < 0) continue;
+      if (threadIdx.x == 0) bulk_store_1d(p.q + (size_t)dest * p.hidden, smem_u32(s_q), (uint32_t)p.hidden);
+      for (int c = threadIdx.x; c < p.kblocks; c += blockDim.x) p.sf[(size_t)c * p.pitch + dest] = s_sf[c];
+    }
+    if (threadIdx.x == 0) bulk_commit_group();    // one group per token (empty ones count too)
+  }
+  if (threadIdx.x == 0) bulk_wait_group0();       // a kernel that starts early follows: the rows are in place
+}
+
 // ---- weights -------------------------------------------------------------------------------
 // A CTA per 128 x 128 block, whose values stay in registers between the maximum and the quotients: a
 // thread holds 64 of them in four row pieces of 16.
@@ -274,6 +348,45 @@ int msc_fp8_block_quantize(const void* x, int x_dtype, int silu, const int32_t* 
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   return x_dtype == 0 ? launch_rows<__nv_bfloat16>(p, silu != 0, st)
          : x_dtype == 1 ? launch_rows<float>(p, silu != 0, st) : launch_rows<__half>(p, silu != 0, st);
+}
+
+int msc_moe_permute_quantize_fp8_block(const void* tokens_bf16, const int32_t* ids, const float* weights,
+                                       const int32_t* rank, const int32_t* group_offsets, int tokens, int hidden,
+                                       int topk, int expert_first, int experts_local, void* a_q, float* a_sf,
+                                       float* row_weight, int32_t* row_token, int rows_cap, void* stream) {
+  using namespace msc;
+  if (!tokens_bf16 || !ids || !weights || !rank || !group_offsets || !a_q || !a_sf || !row_weight || !row_token)
+    return fail(MSC_ERR_BAD_ARG, "NULL pointer");
+  if (tokens < 0 || topk <= 0 || experts_local <= 0 || rows_cap <= 0)
+    return fail(MSC_ERR_BAD_ARG, "tokens must not be negative, topk, experts_local and rows_cap must be positive");
+  if (hidden <= 0 || hidden % 16) return fail(MSC_ERR_BAD_ARG, "hidden=%d must be a positive multiple of 16", hidden);
+  if (topk > kFp8MaxTopk) return fail(MSC_ERR_UNSUPPORTED, "topk=%d exceeds %d", topk, kFp8MaxTopk);
+  if (reinterpret_cast<uintptr_t>(tokens_bf16) % 16 || reinterpret_cast<uintptr_t>(a_q) % 16)
+    return fail(MSC_ERR_BAD_ARG, "tokens and a_q must be 16-byte aligned");
+  for (const void* ptr : {static_cast<const void*>(ids), static_cast<const void*>(weights), static_cast<const void*>(rank),
+                          static_cast<const void*>(group_offsets), static_cast<const void*>(a_sf), static_cast<const void*>(row_weight),
+                          static_cast<const void*>(row_token)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 4) return fail(MSC_ERR_BAD_ARG, "a pointer is not 4-byte aligned");
+  Fp8DispatchParams p;
+  p.tokens = static_cast<const __nv_bfloat16*>(tokens_bf16);
+  p.ids = ids; p.weights = weights; p.rank = rank; p.group_offsets = group_offsets;
+  p.q = static_cast<uint8_t*>(a_q); p.sf = a_sf; p.row_weight = row_weight; p.row_token = row_token;
+  p.hidden = hidden; p.kblocks = (hidden + 127) / 128; p.topk = topk;
+  p.expert_first = expert_first; p.experts_local = experts_local; p.rows_cap = rows_cap; p.pitch = (rows_cap + 3) & ~3;
+  const int smem = 2 * ((hidden + 4 * p.kblocks + 15) & ~15);
+  if (smem > 200 * 1024) return fail(MSC_ERR_UNSUPPORTED, "hidden=%d: two rows do not fit in shared memory", hidden);
+  if (tokens == 0) return MSC_OK;
+  if (smem > 48 * 1024)
+    if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(moe_permute_quantize_fp8_kernel), 200 * 1024)) return rc;
+  const int sms = num_sms();
+  if (sms <= 0) return fail(MSC_ERR_CUDA, "could not query the SM count");
+  // enough CTAs to fill every SM, each walking its share of the tokens; wide CTAs for a few tokens, whose rows
+  // are then one step long
+  const int grid = std::min(tokens, 16 * sms), threads = tokens <= 2 * sms ? 512 : 128;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t lc = pdl_launch_config(grid, threads, smem, static_cast<cudaStream_t>(stream), attr);
+  MSC_CUDA_OK(cudaLaunchKernelEx(&lc, moe_permute_quantize_fp8_kernel, p, tokens));
+  return MSC_OK;
 }
 
 int msc_fp8_block_quantize_weight(const void* w, int w_dtype, void* q, float* sf, int l, int n, int k, void* stream) {

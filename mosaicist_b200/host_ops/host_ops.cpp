@@ -50,7 +50,7 @@ using OptTensor = std::optional<Tensor>;
   X(msc_moe_plan) X(msc_moe_permute_quantize) X(msc_moe_unpermute)                               \
   X(msc_moe_masked_workspace) X(msc_moe_masked) X(msc_moe_route) X(msc_moe_route_backward)       \
   X(msc_fp8_block_quantize) X(msc_fp8_block_quantize_weight) X(msc_gemm_fp8_block)               \
-  X(msc_grouped_gemm_fp8_block_ragged)
+  X(msc_grouped_gemm_fp8_block_ragged) X(msc_moe_permute_quantize_fp8_block)
 
 struct Lib {
 #define X(name) decltype(&::name) name = nullptr;
@@ -1035,6 +1035,47 @@ PY_FUNCTION(moe_dispatch, 3) {
   Py_RETURN_NONE;
 }
 
+// dispatch(self, tokens) of the FP8 block layer: plan, gather + quantise into a_q / a_sf
+PY_FUNCTION(moe_dispatch_fp8_block, 2) {
+  ATTR(ids); ATTR(weights); ATTR(rank); ATTR(group_rows); ATTR(group_offsets); ATTR(total_rows); ATTR(scratch); ATTR(topk);
+  ATTR(E); ATTR(expert_first); ATTR(h); ATTR(a_q); ATTR(a_sf); ATTR(row_weight); ATTR(row_token); ATTR(rows_cap);
+  Layer layer{a[0]};
+  const Tensor& tokens = tensor(a[1], "tokens");
+  const int64_t K = layer.num(s_topk), E = layer.num(s_E), first = layer.num(s_expert_first);
+  const int64_t h = layer.num(s_h), cap = layer.num(s_rows_cap);
+  need_dim(tokens, "tokens", 2);
+  const int64_t T = tokens.size(0);
+  need(tokens, "tokens", kBf16, {T, h});
+  const Tensor &ids = layer.t(s_ids), &weights = layer.t(s_weights), &rank = layer.t(s_rank), &rows = layer.t(s_group_rows);
+  const Tensor &offsets = layer.t(s_group_offsets), &total = layer.t(s_total_rows), &scratch = layer.t(s_scratch);
+  const Tensor &a_q = layer.t(s_a_q), &a_sf = layer.t(s_a_sf), &row_weight = layer.t(s_row_weight), &row_token = layer.t(s_row_token);
+  need_room(ids, "ids", kI32, T * K);
+  need_room(weights, "weights", kF32, T * K);
+  need_room(rank, "rank", kI32, T * K);
+  need_room(rows, "group_rows", kI32, E);
+  need_room(offsets, "group_offsets", kI32, E);
+  need_room(total, "total_rows", kI32, 1);
+  need_room(scratch, "scratch", kI32, 1);
+  need_room(a_q, "a_q", kE4m3, cap * h);
+  need(a_sf, "a_sf", kF32, {blocks_of(h), pitch_of(cap)});
+  need_room(row_weight, "row_weight", kF32, cap);
+  need_room(row_token, "row_token", kI32, cap);
+  one_device(tokens, {{&ids, "ids"}, {&weights, "weights"}, {&rank, "rank"}, {&rows, "group_rows"}, {&offsets, "group_offsets"},
+                      {&total, "total_rows"}, {&scratch, "scratch"}, {&a_q, "a_q"}, {&a_sf, "a_sf"}, {&row_weight, "row_weight"},
+                      {&row_token, "row_token"}});
+  const int t = as_int(T, "tokens"), pairs = as_int(T * K, "tokens * topk");
+  const Lib& f = lib();
+  const OnDeviceOf on(tokens);
+  auto i32 = [](const Tensor& v) { return static_cast<int32_t*>(v.data_ptr()); };
+  launch([&] { return f.msc_moe_plan(i32(ids), pairs, first, E, i32(rank), i32(rows), i32(offsets), i32(total), i32(scratch), on.stream); });
+  launch([&] {
+    return f.msc_moe_permute_quantize_fp8_block(ptr(tokens), i32(ids), ptr<float>(weights), i32(rank), i32(offsets), t, h, K, first, E,
+                                                a_q.data_ptr(), static_cast<float*>(a_sf.data_ptr()),
+                                                static_cast<float*>(row_weight.data_ptr()), i32(row_token), cap, on.stream);
+  });
+  Py_RETURN_NONE;
+}
+
 // combine(self, tokens, out or None) -> out: the sum of each token's expert rows
 PY_FUNCTION(moe_combine, 3) {
   ATTR(y); ATTR(ids); ATTR(rank); ATTR(group_offsets); ATTR(h); ATTR(topk); ATTR(expert_first); ATTR(E);
@@ -1074,6 +1115,7 @@ PyMethodDef kMethods[] = {METHOD(masked_grouped_gemm),
                           METHOD(ragged_grouped_gemm_fp8_block),
                           METHOD(moe_route),
                           METHOD(moe_dispatch),
+                          METHOD(moe_dispatch_fp8_block),
                           METHOD(moe_combine),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_host_ops", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

@@ -10,9 +10,15 @@ SiLU*up + quantise -> GEMM2 (routing weight folded into its epilogue) -> per-tok
 covers the experts [expert_first, expert_first + experts_local) and returns the partial sum
 over those, which is the whole answer on one GPU and one rank's share under expert
 parallelism.
+
+`MegaMoEFp8Block` is the same layer over FP8 weights and activations with fp32 scales per block of 128.  Both
+take a `RouteConfig` for routers that score by sigmoid, carry a load-balancing bias or restrict a token to some
+groups of experts.
 """
 
 from __future__ import annotations
+
+from dataclasses import dataclass
 
 import torch
 
@@ -23,6 +29,23 @@ _host_ops = _lib.native
 
 _OFFSETS = {}
 _DEFAULT_CONFIG = ops.GemmConfig()
+
+
+@dataclass(frozen=True)
+class RouteConfig:
+    """How a routed layer chooses its experts: the arguments of ops.moe_route.  The default is the plain
+    rule, softmax over the experts, the topk largest, weights renormalised."""
+    score: str = "softmax"
+    groups: int = 1
+    topk_groups: int = 1
+    group_top: int = 1
+    renormalize: bool = True
+    scale: float = 1.0
+
+
+def _route(config, logits, topk, bias, out):
+    ops.moe_route(logits, topk, config.score, bias, config.groups, config.topk_groups, config.group_top,
+                  config.renormalize, config.scale, out)
 
 
 def _masked_offsets(l: int, m: int, device) -> torch.Tensor:
@@ -99,10 +122,13 @@ class MegaMoE:
                  topk: int, max_tokens: int, expert_first: int = 0,
                  config: ops.GemmConfig = ops.GemmConfig(), fuse_gemm1: bool = True,
                  rows_cap: int | None = None, workspace: dict | None = None,
-                 gemm1_tokens_on_n: bool | None = None):
+                 gemm1_tokens_on_n: bool | None = None, route: RouteConfig | None = None, route_bias=None):
         """`rows_cap` overrides the row capacity of the grouped buffers (default: room for
         max_tokens * topk rows plus 127 padding rows per expert); `workspace` may provide the
-        buffers other GPUs access under expert parallelism (a_q, a_sf, row_weight, y)."""
+        buffers other GPUs access under expert parallelism (a_q, a_sf, row_weight, y).  `route` and
+        `route_bias` (experts_total,) f32: see RouteConfig; without them the plain rule."""
+        self.route_config = RouteConfig() if route is None and route_bias is not None else route
+        self.route_bias = route_bias
         self.E, n2, hh = w1_q.shape
         self.h, self.n, self.topk = hh * 2, n2 // 2, topk
         self.expert_first, self.config = expert_first, config
@@ -164,7 +190,12 @@ class MegaMoE:
     def route(self, logits):
         """logits (T, experts_total) f32 -> fills ids / weights; returns them."""
         T = logits.shape[0]
-        _host_ops.moe_route(self, logits)
+        if self.route_config is None:
+            _host_ops.moe_route(self, logits)
+        else:
+            if T > self.max_tokens:
+                raise ValueError(f"{T} tokens exceed the workspace built for {self.max_tokens}")
+            _route(self.route_config, logits, self.topk, self.route_bias, (self.ids[:T], self.weights[:T]))
         return self.ids[:T], self.weights[:T]
 
     def forward(self, tokens, logits=None, out=None):
@@ -173,6 +204,11 @@ class MegaMoE:
         T = tokens.shape[0]
         if T > self.max_tokens:
             raise ValueError(f"{T} tokens exceed the workspace built for {self.max_tokens}")
+        if self.route_config is not None and logits is not None:
+            if logits.shape[0] != T:
+                raise ValueError(f"{T} tokens, but logits of {logits.shape[0]}")
+            self.route(logits)
+            logits = None
         _host_ops.moe_dispatch(self, tokens, logits)
         self.run_experts()
         return _host_ops.moe_combine(self, tokens, out)
@@ -196,3 +232,83 @@ class MegaMoE:
                                           self.group_rows, self.alpha1, None, self.config, out=self.gateup)
             ops.quantize_nvfp4_ragged(self.gateup, self.a2_gs, self.group_offsets, self.group_rows,
                                       silu=True, out=(self.d_q, self.d_sf))
+
+
+class MegaMoEFp8Block:
+    """Routed SwiGLU expert layer with e4m3 weights and activations and fp32 scales per block of 128: route ->
+    plan -> gather + quantise -> GEMM1 -> SiLU*up + quantise -> GEMM2 (routing weight folded in) -> per-token sum.
+
+    w1_q (E, 2n, h) e4m3, gate rows first, w1_sf (E, ceil(2n / 128), ceil(h / 128)) f32, w2_q (E, h, n), w2_sf
+    (E, ceil(h / 128), ceil(n / 128)), as ops.quantize_fp8_block_weight makes them, where E is the number of
+    LOCAL experts; h and n are multiples of 16.  Workspaces are sized for `max_tokens` once."""
+
+    def __init__(self, w1_q, w1_sf, w2_q, w2_sf, topk: int, max_tokens: int, expert_first: int = 0,
+                 route: RouteConfig = RouteConfig(), route_bias=None, rows_cap: int | None = None):
+        """`route` and `route_bias` (experts_total,) f32: see RouteConfig.  `rows_cap` overrides the row capacity
+        of the grouped buffers (default: room for max_tokens * topk rows plus 127 padding rows per expert)."""
+        if w1_q.dim() != 3 or w2_q.dim() != 3 or w1_q.shape[1] % 2 or tuple(w2_q.shape) != (
+                w1_q.shape[0], w1_q.shape[2], w1_q.shape[1] // 2):
+            raise ValueError(f"w1_q {tuple(w1_q.shape)} and w2_q {tuple(w2_q.shape)} are not (E, 2n, h) and (E, h, n)")
+        self.E, n2, self.h = w1_q.shape
+        self.n, self.topk, self.expert_first = n2 // 2, topk, expert_first
+        if self.h % 16 or self.n % 16:
+            raise ValueError(f"h={self.h} and n={self.n} must be multiples of 16")
+        if max_tokens < 1 or not 1 <= topk <= 32:
+            raise ValueError("max_tokens must be positive and topk in [1, 32]")
+        self.w1_q, self.w1_sf, self.w2_q, self.w2_sf = w1_q, w1_sf, w2_q, w2_sf
+        self.route_config, self.route_bias = route, route_bias
+        self.max_tokens = max_tokens
+        cap = rows_cap if rows_cap is not None else (max_tokens * topk + 127 * self.E + 127) // 128 * 128
+        if cap <= 0 or cap % 128:
+            raise ValueError(f"rows_cap={cap} must be a positive multiple of 128")
+        self.rows_cap = cap
+        on = dict(device=w1_q.device)
+        i32, f32, u8, bf16 = (dict(dtype=d, **on) for d in (torch.int32, torch.float32, torch.uint8, torch.bfloat16))
+        self.ids = torch.zeros((max_tokens, topk), **i32)
+        self.weights = torch.zeros((max_tokens, topk), **f32)
+        self.rank = torch.zeros((max_tokens, topk), **i32)
+        self.group_rows = torch.zeros((self.E,), **i32)
+        self.group_offsets = torch.zeros((self.E,), **i32)
+        self.total_rows = torch.zeros((1,), **i32)
+        self.scratch = torch.zeros((4,), **i32)
+        self.a_q = torch.empty((cap, self.h), **u8)
+        self.a_sf = torch.zeros(((self.h + 127) // 128, cap), **f32)
+        self.row_weight = torch.zeros((cap,), **f32)
+        self.row_token = torch.zeros((cap,), **i32)
+        self.gateup = torch.empty((cap, n2), **bf16)
+        self.d_q = torch.empty((cap, self.n), **u8)
+        self.d_sf = torch.zeros(((self.n + 127) // 128, cap), **f32)
+        self.y = torch.empty((cap, self.h), **bf16)
+
+    def route(self, logits):
+        """logits (T, experts_total) bf16 / f16 / f32 -> fills ids / weights; returns them."""
+        T = logits.shape[0]
+        if T > self.max_tokens:
+            raise ValueError(f"{T} tokens exceed the workspace built for {self.max_tokens}")
+        out = self.ids[:T], self.weights[:T]
+        _route(self.route_config, logits, self.topk, self.route_bias, out)
+        return out
+
+    def forward(self, tokens, logits=None, out=None):
+        """tokens (T, h) bf16; logits (T, experts_total), or None to reuse the routing already in self.ids /
+        self.weights.  Returns (T, h) bf16, the sum over the local experts."""
+        T = tokens.shape[0]
+        if T > self.max_tokens:
+            raise ValueError(f"{T} tokens exceed the workspace built for {self.max_tokens}")
+        if logits is not None:
+            if logits.shape[0] != T:
+                raise ValueError(f"{T} tokens, but logits of {logits.shape[0]}")
+            self.route(logits)
+        if T == 0:
+            return torch.empty((0, self.h), dtype=torch.bfloat16, device=tokens.device) if out is None else out
+        _host_ops.moe_dispatch_fp8_block(self, tokens)
+        self.run_experts()
+        return _host_ops.moe_combine(self, tokens, out)
+
+    def run_experts(self):
+        """GEMM1 -> SiLU*up + quantise -> GEMM2 over the grouped rows in a_q / a_sf, result rows times row_weight
+        into y."""
+        groups = self.group_offsets, self.group_rows
+        ops.ragged_grouped_gemm_fp8_block(self.a_q, self.a_sf, self.w1_q, self.w1_sf, *groups, out=self.gateup)
+        ops.quantize_fp8_block(self.gateup, True, *groups, out=(self.d_q, self.d_sf))
+        ops.ragged_grouped_gemm_fp8_block(self.d_q, self.d_sf, self.w2_q, self.w2_sf, *groups, self.row_weight, out=self.y)

@@ -194,3 +194,53 @@ def test_operators_can_be_traced(fake):
     ids, w = O.moe_route(_t(10, 64), 4, "sigmoid", None, 1, 1, 1, True, 1.0)
     assert ids.dtype == I32 and w.shape == (10, 4)
     assert O.moe_route_backward(w, _t(10, 64, dtype=F16), ids, w, "sigmoid", True, 1.0).dtype == F16
+
+
+@pytest.mark.parametrize("kw", [
+    dict(tokens_ptr=None), dict(ids=None), dict(w=None), dict(rank=None), dict(offs=None), dict(a_q=None), dict(a_sf=None), dict(rw=None), dict(rt=None),
+    dict(tokens=-1), dict(hidden=0), dict(hidden=100), dict(topk=0), dict(topk=65), dict(local=0), dict(cap=0), dict(tokens_ptr=P + 2), dict(a_q=P + 8),
+    dict(a_sf=P + 2), dict(ids=P + 1), dict(hidden=200000)])
+def test_dispatch_refusals(lib, kw):
+    a = dict(tokens_ptr=P, ids=P, w=P, rank=P, offs=P, tokens=8, hidden=256, topk=2, first=0, local=4, a_q=P, a_sf=P, rw=P, rt=P, cap=512) | kw
+    assert lib.msc_moe_permute_quantize_fp8_block(*a.values(), None) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
+
+
+def _layer_stub(**kw):
+    from types import SimpleNamespace
+
+    T, K, E, h, cap = 16, 2, 8, 272, 1152
+    i32 = lambda *s: _t(*s, dtype=I32)
+    return SimpleNamespace(**(dict(
+        ids=i32(T, K), weights=_t(T, K), rank=i32(T, K), group_rows=i32(E), group_offsets=i32(E), total_rows=i32(1), scratch=i32(4), topk=K, E=E,
+        expert_first=0, h=h, a_q=_t(cap, h, dtype=U8), a_sf=_t(3, cap), row_weight=_t(cap), row_token=i32(cap), rows_cap=cap) | kw))
+
+
+def test_fp8_layer_buffers(fake):
+    from mosaicist_b200.moe import _host_ops
+
+    x = _t(16, 272, dtype=BF16)
+    for kw in (dict(ids=_t(15, 2, dtype=I32)), dict(weights=_t(16, 2, dtype=BF16)), dict(rank=_t(16, 1, dtype=I32)), dict(a_q=_t(1151, 272, dtype=U8)),
+               dict(a_sf=_t(2, 1152)), dict(a_sf=_t(3, 1148)), dict(row_weight=_t(1151)), dict(row_token=_t(1152)), dict(group_rows=_t(7, dtype=I32)),
+               dict(a_q=_t(1152, 272, dtype=U8, device="cuda:1")), dict(row_weight=None)):
+        with pytest.raises(ValueError):
+            _host_ops.moe_dispatch_fp8_block(_layer_stub(**kw), x)
+    for bad in (_t(17, 272, dtype=BF16), _t(16, 256, dtype=BF16), _t(16, 272), _t(16, 272, dtype=BF16, device="cpu"), _t(272, 16, dtype=BF16).t()):
+        with pytest.raises(ValueError):
+            _host_ops.moe_dispatch_fp8_block(_layer_stub(), bad)
+
+
+def test_fp8_layer_arguments(fake):
+    from mosaicist_b200.moe import MegaMoEFp8Block
+
+    w1, s1, w2, s2 = _t(4, 512, 256, dtype=U8), _t(4, 4, 2), _t(4, 256, 256, dtype=U8), _t(4, 2, 2)
+    layer = MegaMoEFp8Block(w1, s1, w2, s2, topk=2, max_tokens=8)
+    assert layer.rows_cap == 640 and layer.a_sf.shape == (2, 640)
+    for kw in (dict(topk=0), dict(topk=33), dict(max_tokens=0), dict(rows_cap=100), dict(rows_cap=0)):
+        with pytest.raises(ValueError):
+            MegaMoEFp8Block(w1, s1, w2, s2, **(dict(topk=2, max_tokens=8) | kw))
+    for a, b in ((w1[0], w2), (w1, w2[:3]), (w1[:, :511], w2), (_t(4, 512, 248, dtype=U8), _t(4, 248, 256, dtype=U8)), (w1, _t(4, 256, 128, dtype=U8))):
+        with pytest.raises(ValueError):
+            MegaMoEFp8Block(a, s1, b, s2, topk=2, max_tokens=8)
+    for call in (lambda: layer.forward(_t(9, 256, dtype=BF16)), lambda: layer.route(_t(9, 4)), lambda: layer.forward(_t(8, 256, dtype=BF16), _t(7, 4))):
+        with pytest.raises(ValueError):
+            call()
