@@ -9,14 +9,20 @@
 //
 // What a choice has to be.  The order of the keys is that of 64-bit arithmetic.  Without a bias and with
 // groups judged by their best expert the order of the keys is the order of the logits, and nothing is
-// rounded.  Otherwise the keys are computed in fp32, whose error is bounded (key_tolerance below); a
-// token in which two keys that the result tells apart lie closer than that is chosen over again in 64
-// bits (about one token in a thousand for 256 experts).
+// rounded.  Otherwise the keys are computed in fp32, whose error is bounded (`tol` below); a token in which two
+// keys that the result tells apart lie closer than that is looked at again in 64 bits (about one token in a
+// thousand for 256 experts).
 //
-// Layout: a warp per token, the experts of a group spread over the lanes, 32 to a register slot, so that
-// a group's maximum is one warp reduction (redux.sync) per slot; groups of fewer than 32 experts leave
-// lanes idle.  A thread-wide maximum over the slots, one reduction and one minimum over the experts that
-// hold it make a choice; 256 experts, top 8 of 4 of 8 groups take about 700 instructions per token.
+// Two layouts.  A warp per token, the experts of a group spread over the lanes, 32 to a register slot: a group's
+// maximum is one warp reduction (redux.sync) per slot, and a thread-wide maximum over the slots, one reduction and
+// one minimum over the experts that hold it make a choice.  That is the shortest way for a few tokens and serves up
+// to 1024 experts, but 256 experts, top 8 of 4 of 8 groups take about 1330 instructions per token, most of
+// them the serial rounds of choosing.  From 1024 tokens on, and up to 256 experts, eight lanes per token share
+// these rounds among four tokens (below).
+//
+// Neither is bound by memory: 8192 tokens of 256 fp32 logits are 8.9 MB, 1.4 us, and take 12 us with sigmoid,
+// bias and 4 of 8 groups (21 a warp per token), 5 us for 128 bf16 experts without them; 16 tokens take 4.5 us. What is left
+// is the chain of one warp's steps (3 to 4 us) and, where keys lie close, the tokens that are looked at in 64 bits.
 //
 // A logit of -inf or NaN, or a bias of -inf or NaN, bars its expert.  Where fewer than topk experts are
 // left, the lowest barred ones fill up the ids (they stay distinct and in range) with weight 0.
@@ -25,6 +31,8 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <cfloat>
 
 namespace msc {
 
@@ -38,8 +46,12 @@ struct RouteParams {
   int per, slots;        // experts and register slots of a group
   int base[32];          // lane 0's expert of every slot
   int renormalize;
+  int sigmoid;           // else softmax
   int by_score;          // keys are scores (+ bias), else logits
   float scale;
+  // eight lanes a token
+  int lanes, chunk;      // lanes of a group, experts of a lane (the last lane of a group may have fewer)
+  int per_inv, chunk_inv;   // ceil(2^16 / .): exact quotients of numbers below 256 by a multiplication
 };
 
 __device__ __forceinline__ float as_float(float v) { return v; }
@@ -293,6 +305,33 @@ __device__ __noinline__ Pick choose_in_64_bits(const RouteParams& p, const T* ro
   return pick;
 }
 
+__device__ __forceinline__ float sigmoid_weight(float x) {
+  const float e = expf(-fabsf(x));
+  return x >= 0.0f ? __fdiv_rn(1.0f, 1.0f + e) : __fdiv_rn(e, 1.0f + e);
+}
+__device__ __forceinline__ float softmax_weight(float x, float ref) {
+  return x == ref ? (x == -INFINITY ? 0.0f : 1.0f) : expf(x - ref);
+}
+
+// Sigmoids of so small a logit, e^x each, vanish in fp32 but not in 64 bits: their ratios are e^(x - best).
+__device__ __forceinline__ bool vanishing(float best) { return best < -64.0f && best >= -709.7827f; }
+
+// A bit per slot in which this lane has an expert.
+template <int PER>
+__device__ __forceinline__ uint32_t open_slots(const RouteParams& p, int lane) {
+  uint32_t open = 0;
+  int j = 0, g = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (g < p.groups && j * 32 + lane < p.per) open |= 1u << i;
+    if (++j == p.slots) {
+      j = 0;
+      ++g;
+    }
+  }
+  return open;
+}
+
 template <int PER, bool SIGMOID, class T>
 __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
   __shared__ int base[32];
@@ -306,19 +345,11 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
   const T* row = static_cast<const T*>(p.logits) + token * p.experts;
 
   float key[PER], b[PER];
-  uint32_t open = 0;
-  {
-    int j = 0, g = 0;
+  const uint32_t open = open_slots<PER>(p, lane);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      if (g < p.groups && j * 32 + lane < p.per) open |= 1u << i;
-      key[i] = ((open >> i) & 1u) ? load_logit(row + base[i] + lane) : -INFINITY;
-      b[i] = (p.bias && ((open >> i) & 1u)) ? ld_ordered(p.bias + base[i] + lane) : 0.0f;
-      if (++j == p.slots) {
-        j = 0;
-        ++g;
-      }
-    }
+  for (int i = 0; i < PER; ++i) {
+    key[i] = ((open >> i) & 1u) ? load_logit(row + base[i] + lane) : -INFINITY;
+    b[i] = (p.bias && ((open >> i) & 1u)) ? ld_ordered(p.bias + base[i] + lane) : 0.0f;
   }
   float mx = -INFINITY, sum = 0.0f;
   if (!SIGMOID && (p.by_score || !p.renormalize)) {
@@ -358,11 +389,13 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
   const float x = there ? load_logit(row + pick.id) : -INFINITY;
   float w;
   if (SIGMOID) {
-    const float e = expf(-fabsf(x));
-    w = x >= 0.0f ? __fdiv_rn(1.0f, 1.0f + e) : __fdiv_rn(e, 1.0f + e);
+    w = sigmoid_weight(x);
+    if (p.renormalize) {
+      const float best = warp_max(x);
+      if (vanishing(best)) w = softmax_weight(x, best);
+    }
   } else {
-    const float ref = p.renormalize ? warp_max(x) : mx;   // a common factor of the chosen ones cancels
-    w = x == ref ? (x == -INFINITY ? 0.0f : 1.0f) : expf(x - ref);
+    w = softmax_weight(x, p.renormalize ? warp_max(x) : mx);   // a common factor of the chosen ones cancels
     if (!p.renormalize) w = sum > 0.0f ? __fdiv_rn(w, sum) : 0.0f;
   }
   if (!there) w = 0.0f;
@@ -373,6 +406,318 @@ __global__ void __launch_bounds__(128) moe_route_kernel(const RouteParams p) {
   if (lane < p.topk) {
     p.ids[token * p.topk + lane] = pick.id;
     p.weights[token * p.topk + lane] = w * p.scale;
+  }
+}
+
+// ---- eight lanes a token ---------------------------------------------------------------------
+// Up to 256 experts in 1, 2, 4 or 8 groups, topk <= 8: a warp takes four tokens, eight lanes each, and a lane
+// up to 32 experts of one group.  A key is an unsigned word in the order of the keys, its lowest 8 bits
+// 255 - expert, so that words are distinct and ties fall to the lower expert.  Lanes sort theirs in eights by
+// networks, and three exchanges merge the best eight of the lanes; nothing branches.
+//   Logits: the upper 24 bits of the fp32 number (all that a 16-bit logit has).
+//   Scores: 23 bits of fixed point over [largest bias - 8, largest score + largest bias], or less where the
+//   biases span less; a key below counts as the window's lower end.
+// From this many tokens on.  A warp of four tokens takes longer than a warp of one (E = experts, us at 16 / 1024 /
+// 2048 / 8192 tokens, eight lanes against a warp a token): E = 61 2.6 / 3.2 / 3.3 / 4.9 against 1.9 / 3.1 / 3.9 / 9.6;
+// E = 128 2.4 / 2.7 / 2.8 / 4.8 against 2.3 / 3.2 / 4.1 / 11.3; E = 160 in groups 3.7 / 4.0 / 4.2 / 7.0 against
+// 3.1 / 4.1 / 5.2 / 13.7.
+constexpr int kOctetTokens = 1024;
+constexpr int kOctetWarps = 2;
+constexpr float kWindow = 8.0f, kUnits = 0x1p23f - 32.0f;
+
+enum { kByLogit = 0, kBySoftmax = 1, kBySigmoid = 2 };   // what the keys are
+
+template <int KEYS>
+struct Word {
+  // words below it are those of -inf: barred
+  static constexpr uint32_t kLeast = KEYS == kByLogit ? 0x00800000u : 1u << 9;
+  // `v`: a logit, or a place in the window, 2^23 + 1 .. 2^24 - 1 where it is not below it
+  static __device__ __forceinline__ uint32_t of(float v, uint32_t low) {
+    if (KEYS == kByLogit) {
+      const uint32_t bits = __float_as_uint(v);
+      return ((bits ^ ((uint32_t)((int)bits >> 31) | 0x80000000u)) & ~255u) | (low & 255u);
+    }
+    return v == -INFINITY ? 0u : (__float_as_uint(fmaxf(v, 0x1p23f + 1.0f)) << 9) | (low & 255u);
+  }
+  // The logit or at most 2^-15 of it less; the place less 2^24.
+  static __device__ __forceinline__ float value(uint32_t word) {
+    const uint32_t o = word & ~255u;
+    if (word < kLeast) return -INFINITY;
+    return KEYS == kByLogit ? __uint_as_float(o ^ ((int)o < 0 ? 0x80000000u : 0xffffffffu)) : __uint_as_float((o >> 9) | 0x4b000000u) - 0x1p24f;
+  }
+  static __device__ __forceinline__ bool below_window(uint32_t word) { return KEYS != kByLogit && word < 2u << 9; }
+};
+__device__ __forceinline__ void order(uint32_t& a, uint32_t& b) {
+  const uint32_t hi = max(a, b);
+  b = min(a, b);
+  a = hi;
+}
+__device__ __forceinline__ void sort8(uint32_t* v) {   // falling (Batcher's odd-even merging)
+  order(v[0], v[1]); order(v[2], v[3]); order(v[4], v[5]); order(v[6], v[7]);
+  order(v[0], v[2]); order(v[1], v[3]); order(v[4], v[6]); order(v[5], v[7]);
+  order(v[1], v[2]); order(v[5], v[6]);
+  order(v[0], v[4]); order(v[1], v[5]); order(v[2], v[6]); order(v[3], v[7]);
+  order(v[2], v[4]); order(v[3], v[5]);
+  order(v[1], v[2]); order(v[3], v[4]); order(v[5], v[6]);
+}
+// v: the best eight of two falling lists; `left`: the best word that was dropped.
+template <bool CHECK>
+__device__ __forceinline__ void merge8(uint32_t* v, const uint32_t* with, uint32_t& left) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (CHECK) left = max(left, min(v[i], with[7 - i]));
+    v[i] = max(v[i], with[7 - i]);
+  }
+#pragma unroll
+  for (int d = 4; d; d >>= 1)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (!(i & d)) order(v[i], v[i + d]);
+}
+template <class F>
+__device__ __forceinline__ F octet_sum(F v) {
+#pragma unroll
+  for (int o = 4; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ float octet_max(float v) {
+#pragma unroll
+  for (int o = 4; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+template <int PER, int KEYS, class T>
+__global__ void __launch_bounds__(32 * kOctetWarps) moe_route_octets_kernel(const RouteParams p) {
+  constexpr int kPitch = PER + 1, kTokenPitch = 8 * kPitch;   // the 32 lanes' k-th words lie in 32 banks
+  constexpr bool kCheck = KEYS != kByLogit || sizeof(T) == 4;   // a 16-bit logit keeps all its bits in a word
+  __shared__ float s_rows[kOctetWarps][4 * kTokenPitch];
+  __shared__ float s_bias[KEYS == kByLogit ? 1 : kOctetWarps][kTokenPitch];
+  __shared__ int s_some[kOctetWarps][32];
+  using W = Word<KEYS>;
+  __shared__ int base[32];
+  base[threadIdx.x & 31] = p.base[threadIdx.x & 31];   // (every warp the same)
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & 7, quad = lane >> 3;
+  float* s_x = s_rows[warp];
+  // where the logit of an expert lies in a token's row
+  auto at = [&](int e) {
+    const int g = (e * p.per_inv) >> 16, j = e - g * p.per;
+    const int h = (j * p.chunk_inv) >> 16;
+    return (g * p.lanes + h) * kPitch + (j - h * p.chunk);
+  };
+  const int group = sub / p.lanes, first = sub - group * p.lanes;        // this lane's
+  const int e0 = group * p.per + first * p.chunk;
+  const int count = min(max(p.per - first * p.chunk, 0), p.chunk);
+  const float* list = s_x + quad * kTokenPitch + sub * kPitch;
+  for (int i = count; i < PER; ++i) s_x[quad * kTokenPitch + sub * kPitch + i] = -INFINITY;
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const long long token0 = ((long long)blockIdx.x * kOctetWarps + warp) * 4;
+  const T* rows = static_cast<const T*>(p.logits) + token0 * p.experts;
+  const int tokens = (int)min(max(p.tokens - token0, 0LL), 4LL);         // of this warp
+  for (int c = lane; c < p.experts; c += 128) {
+    float v[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        v[i][q] = (c + 32 * i < p.experts && q < tokens) ? load_logit(rows + q * p.experts + c + 32 * i) : -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + 32 * i < p.experts) {
+        const int to = at(c + 32 * i);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s_x[q * kTokenPitch + to] = v[i][q] + 0.0f;   // (-0 counts as 0)
+      }
+  }
+  float spread = 0.0f;          // the biases' part of the window
+  bool hopeless = false;
+  if (KEYS != kByLogit) {       // biases less the largest one
+    float b[8], most = p.bias ? -INFINITY : 0.0f, least = INFINITY;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = lane + 32 * i;
+      b[i] = e >= p.experts ? -INFINITY : p.bias ? ld_ordered(p.bias + e) : 0.0f;
+      if (b[i] > -INFINITY) {   // (a NaN is not)
+        most = fmaxf(most, b[i]);
+        least = fminf(least, b[i]);
+      } else {
+        b[i] = -INFINITY;
+      }
+    }
+    most = warp_max(most);
+    least = -warp_max(-least);
+    hopeless = !(fabsf(most) <= FLT_MAX);
+    spread = fminf(most - least, kWindow);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < p.experts) s_bias[warp][at(lane + 32 * i)] = b[i] > -INFINITY ? fmaxf(b[i] - most, -1e20f) : b[i];
+  }
+  __syncwarp();
+  if (tokens == 0) return;
+
+  const bool softmax = KEYS == kBySoftmax || (KEYS == kByLogit && !p.sigmoid);
+  float mx = -INFINITY, sum = 0.0f, inv = 0.0f;
+  if (KEYS == kBySoftmax || (KEYS == kByLogit && softmax && !p.renormalize)) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) mx = fmaxf(mx, list[i]);
+    mx = octet_max(mx);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sum += exp_below(list[i], mx);
+    sum = octet_sum(sum);
+    inv = sum > 0.0f ? __fdividef(1.0f, sum) : 0.0f;
+  }
+  const float top = KEYS == kBySoftmax && sum > 0.0f ? inv : 1.0f;       // the largest score there can be
+  const float unit = __fdividef(kUnits, top + spread), end = 0x1p24f - 16.0f - top * unit;
+  uint32_t word[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const float x = list[i];
+    float v = x;
+    if (KEYS != kByLogit) {
+      const float s = KEYS == kBySigmoid ? sigmoid(x) : exp_below(x, mx) * inv;
+      v = x == -INFINITY ? -INFINITY : fmaf(s + s_bias[warp][sub * kPitch + i], unit, end);
+    }
+    word[i] = W::of(v, (uint32_t)(255 - e0 - i));
+  }
+  uint32_t left = 0;
+  sort8(word);
+#pragma unroll
+  for (int b = 8; b < PER; b += 8) {
+    sort8(word + b);
+    merge8<kCheck>(word, word + b, left);
+  }
+  // What the difference of two keys may be off by, in units: that of the scores (as above), 2 from rounding
+  // the bias' distance and the sum, 1 from the place itself.  Of two logits that differ in their words none is mistaken.
+  const float tol = KEYS == kByLogit ? 0.0f : (KEYS == kBySigmoid ? 0x1p-20f : 0x1p-17f * inv) * unit + 4.0f;
+  bool near = false, kept = true;      // this lane's group
+  if (p.groups > 1) {
+    uint32_t a = word[0], b = word[1];
+    for (int o = 1; o < p.lanes; o <<= 1) {
+      const uint32_t a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+      b = max(min(a, a2), max(b, b2));
+      a = max(a, a2);
+    }
+    const float best = W::value(a), second = p.group_top == 2 ? W::value(b) : 0.0f;
+    const float strength = (best == -INFINITY || second == -INFINITY) ? -INFINITY : best + second;
+    int ahead = 0;
+#pragma unroll
+    for (int o = 0; o < 8; ++o) {
+      const float other = __shfl_sync(0xffffffffu, strength, o, 8);
+      if ((o & (p.lanes - 1)) == 0) ahead += (other > strength || (other == strength && o < sub - first)) ? 1 : 0;
+    }
+    kept = ahead < p.topk_groups;
+    if (kCheck) {
+      const float weakest = -octet_max(kept ? -strength : -INFINITY), out = octet_max(kept ? -INFINITY : strength);
+      near = out != -INFINITY && !(weakest - out > tol * p.group_top);
+      // (of a group that is kept for a key below the window nothing is known)
+      const float unknown = octet_max(kept && strength != -INFINITY && W::below_window(p.group_top == 2 ? b : a) ? 1.0f : 0.0f);
+      near = near || unknown > 0.0f;
+    }
+    if (!kept) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) word[i] = 0;
+      left = 0;
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    uint32_t with[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) with[i] = __shfl_xor_sync(0xffffffffu, word[i], o);
+    if (kCheck) left = max(left, __shfl_xor_sync(0xffffffffu, left, o));
+    merge8<kCheck>(word, with, left);
+  }
+  uint32_t mine = word[0];               // lane k has the k-th choice
+#pragma unroll
+  for (int i = 1; i < 8; ++i) mine = sub == i ? word[i] : mine;
+  bool again = near || hopeless || (sub < p.topk && mine < W::kLeast);
+  bool close = false;                    // only choices that are certain to be of the groups chosen
+  if (kCheck) {
+    const uint32_t following = __shfl_down_sync(0xffffffffu, mine, 1, 8);
+    const float a = W::value(mine), b = W::value(sub == 7 ? left : following);
+    if (sub < p.topk && b != -INFINITY) close = !(a - b > tol);
+    if (KEYS == kBySoftmax) again = again || close;   // its 64-bit score takes every expert
+  }
+  Pick pick;
+  pick.id = 255 - (int)(mine & 255u);
+  pick.barred = false;
+  uint32_t redo = __ballot_sync(0xffffffffu, again && quad < tokens);
+  if (kCheck && KEYS != kBySoftmax) {
+    uint32_t part = __ballot_sync(0xffffffffu, close && quad < tokens);
+    while (part) {                       // of a token: what comes into question, a lane each, ranked in 64 bits
+      const int q = (__ffs(part) - 1) >> 3;
+      const uint32_t octet = 0xffu << (8 * q);
+      part &= ~octet;
+      if (redo & octet) continue;
+      const float cut = __shfl_sync(0xffffffffu, W::value(mine), 8 * q + p.topk - 1) - 2.0f * tol;
+      const bool in = __shfl_sync(0xffffffffu, (int)kept, 8 * q + sub) != 0;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < PER / 4; ++i) {
+        const int slot = quad * (PER / 4) + i;
+        const float x = s_x[q * kTokenPitch + sub * kPitch + slot];
+        float v = x;
+        if (KEYS != kByLogit && x != -INFINITY)
+          v = fmaxf(fmaf(sigmoid(x) + s_bias[warp][sub * kPitch + slot], unit, end), 0x1p23f + 1.0f) - 0x1p24f;
+        const uint32_t who = __ballot_sync(0xffffffffu, in && v >= cut);
+        const int place = n + __popc(who & ((1u << lane) - 1u));
+        if (in && v >= cut && place < 32) s_some[warp][place] = e0 + slot;
+        n += __popc(who);
+      }
+      __syncwarp();
+      if (n < p.topk || n > 32) {
+        redo |= octet;
+      } else {
+        const int e = s_some[warp][min(lane, n - 1)];
+        double key = s_x[q * kTokenPitch + at(e)];
+        if (KEYS != kByLogit) key = sigmoid(key) + (p.bias ? (double)ld_ordered(p.bias + e) : 0.0);
+        int ahead = 0;
+        for (int o = 0; o < n; ++o) {
+          const double other = __shfl_sync(0xffffffffu, key, o);
+          const int oe = __shfl_sync(0xffffffffu, e, o);
+          ahead += (other > key || (other == key && oe < e)) ? 1 : 0;
+        }
+        __syncwarp();
+        if (lane < n) s_some[warp][ahead] = e;
+        __syncwarp();
+        if (quad == q) pick.id = s_some[warp][sub];
+      }
+      __syncwarp();
+    }
+  }
+  while (redo) {
+    const int q = (__ffs(redo) - 1) >> 3;
+    const Pick found = choose_in_64_bits<8, KEYS == kBySigmoid, T>(p, rows + q * p.experts, open_slots<8>(p, lane), base, lane);
+    const int id = __shfl_sync(0xffffffffu, found.id, sub);
+    const bool barred = __shfl_sync(0xffffffffu, (int)found.barred, sub) != 0;
+    if (quad == q) {
+      pick.id = id;
+      pick.barred = barred;
+    }
+    redo &= ~(0xffu << (8 * q));
+  }
+  const bool there = sub < p.topk && !pick.barred && quad < tokens;
+  const float x = there ? s_x[quad * kTokenPitch + at(pick.id)] : -INFINITY;
+  float w;
+  if (!softmax) {
+    w = sigmoid_weight(x);
+    if (p.renormalize) {
+      const float best = octet_max(x);
+      if (vanishing(best)) w = softmax_weight(x, best);
+    }
+  } else {
+    w = softmax_weight(x, p.renormalize ? octet_max(x) : mx);   // a common factor of the chosen ones cancels
+    if (!p.renormalize) w = sum > 0.0f ? __fdiv_rn(w, sum) : 0.0f;
+  }
+  if (!there) w = 0.0f;
+  if (p.renormalize) {
+    const float all = octet_sum(w);
+    w = all > 0.0f ? __fdiv_rn(w, all) : 0.0f;
+  }
+  if (sub < p.topk && quad < tokens) {
+    const long long to = (token0 + quad) * p.topk + sub;
+    p.ids[to] = pick.id;
+    p.weights[to] = w * p.scale;
   }
 }
 
@@ -391,7 +736,7 @@ struct RouteBackwardParams {
   const float* grad_weights;  // (tokens, topk)
   void* grad_logits;          // (tokens, experts)
   int tokens, experts, topk, renormalize;
-  float inv_scale;
+  float scale;
 };
 
 constexpr int kBackwardWarps = 4;
@@ -420,7 +765,7 @@ __global__ void __launch_bounds__(32 * kBackwardWarps) moe_route_backward_kernel
   }
   if (w == 0.0f) g = 0.0f;   // an infinite gradient of a weight that does not move
   const float all = warp_sum(g * w);
-  float c = w * (p.renormalize ? g - all * p.inv_scale : g);
+  float c = w * (p.renormalize ? g - __fdiv_rn(all, p.scale) : g);
   if (SIGMOID && id >= 0) c *= __fdiv_rn(1.0f, 1.0f + expf(load_logit(row + id)));
 
   if (!SIGMOID && !p.renormalize) {
@@ -463,6 +808,32 @@ static int launch_route(const RouteParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t lc = pdl_launch_config((p.tokens - 1) / 4 + 1, 128, 0, stream, attr);
   MSC_CUDA_OK(cudaLaunchKernelEx(&lc, kern, p));
   return MSC_OK;
+}
+
+template <int KEYS, class T>
+static int launch_octets(const RouteParams& p, cudaStream_t stream) {
+  auto kern = p.chunk <= 8 ? moe_route_octets_kernel<8, KEYS, T>
+              : p.chunk <= 16 ? moe_route_octets_kernel<16, KEYS, T>
+              : p.chunk <= 24 ? moe_route_octets_kernel<24, KEYS, T> : moe_route_octets_kernel<32, KEYS, T>;
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t lc = pdl_launch_config((p.tokens - 1) / (4 * kOctetWarps) + 1, 32 * kOctetWarps, 0, stream, attr);
+  MSC_CUDA_OK(cudaLaunchKernelEx(&lc, kern, p));
+  return MSC_OK;
+}
+
+template <class T>
+static int launch_route_of(RouteParams& p, cudaStream_t stream) {
+  // (words have 8 bits for the expert; a lane's groups would not be its own if they were more than lanes)
+  const bool eights = p.experts <= 256 && p.topk <= 8 && p.groups <= 8 && (p.groups & (p.groups - 1)) == 0;
+  if (eights && p.tokens >= kOctetTokens) {
+    p.lanes = 8 / p.groups;
+    p.chunk = (p.per + p.lanes - 1) / p.lanes;
+    p.per_inv = (0x10000 + p.per - 1) / p.per;
+    p.chunk_inv = (0x10000 + p.chunk - 1) / p.chunk;
+    return !p.by_score ? launch_octets<kByLogit, T>(p, stream)
+           : p.sigmoid ? launch_octets<kBySigmoid, T>(p, stream) : launch_octets<kBySoftmax, T>(p, stream);
+  }
+  return p.sigmoid ? launch_route<true, T>(p, stream) : launch_route<false, T>(p, stream);
 }
 
 template <bool SIGMOID, class T>
@@ -524,15 +895,12 @@ int msc_moe_route(const void* logits, int dtype, const float* bias, int32_t* ids
                 groups, per);
   for (int i = 0; i < 32; ++i) p.base[i] = i / p.slots * p.per + i % p.slots * 32;
   p.renormalize = cfg->renormalize != 0;
+  p.sigmoid = cfg->score == MSC_SCORE_SIGMOID;
   p.by_score = bias != nullptr || (limited && cfg->group_top == 2);
   p.scale = cfg->scale;
   if (tokens == 0) return MSC_OK;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (cfg->score == MSC_SCORE_SIGMOID)
-    return dtype == 0 ? launch_route<true, __nv_bfloat16>(p, st) : dtype == 1 ? launch_route<true, float>(p, st)
-                                                                             : launch_route<true, __half>(p, st);
-  return dtype == 0 ? launch_route<false, __nv_bfloat16>(p, st) : dtype == 1 ? launch_route<false, float>(p, st)
-                                                                            : launch_route<false, __half>(p, st);
+  return dtype == 0 ? launch_route_of<__nv_bfloat16>(p, st) : dtype == 1 ? launch_route_of<float>(p, st) : launch_route_of<__half>(p, st);
 }
 
 int msc_moe_route_backward(const float* grad_weights, const void* logits, int dtype, const int32_t* ids,
@@ -546,7 +914,7 @@ int msc_moe_route_backward(const float* grad_weights, const void* logits, int dt
   RouteBackwardParams p;
   p.logits = logits; p.ids = ids; p.weights = weights; p.grad_weights = grad_weights; p.grad_logits = grad_logits;
   p.tokens = tokens; p.experts = experts; p.topk = topk; p.renormalize = renormalize != 0;
-  p.inv_scale = 1.0f / scale;
+  p.scale = scale;
   if (tokens == 0) return MSC_OK;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (score == MSC_SCORE_SIGMOID)

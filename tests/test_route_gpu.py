@@ -275,3 +275,171 @@ def test_the_layers_own_routing_is_the_plain_case():
     got = ops.moe_route(x, 8)
     assert torch.equal(got[0], ids)
     assert (got[1] - w).abs().max() <= 2e-6
+
+
+# From 1024 tokens on eight lanes share a token of up to 256 experts (1, 2, 4 or 8 groups, topk up to 8).
+MANY = [  # experts, topk, groups, topk_groups, group_top
+    (1, 1, 1, 1, 1), (2, 2, 1, 1, 1), (7, 3, 1, 1, 1), (8, 8, 8, 8, 1), (8, 4, 8, 5, 1), (16, 3, 2, 1, 2), (31, 5, 1, 1, 1), (61, 4, 1, 1, 1),
+    (64, 8, 4, 2, 2), (100, 7, 4, 3, 2), (128, 8, 1, 1, 1), (130, 6, 2, 1, 2), (160, 6, 8, 3, 1), (160, 8, 8, 3, 2), (200, 1, 8, 1, 2), (250, 8, 2, 1, 1),
+    (255, 7, 1, 1, 1), (256, 8, 8, 4, 2), (256, 8, 8, 1, 2), (256, 8, 4, 2, 1), (256, 1, 1, 1, 1)]
+
+
+@pytest.mark.parametrize("score,biased,renormalize", list(itertools.product(["softmax", "sigmoid"], [False, True], [True, False])))
+@pytest.mark.parametrize("E,k,G,tg,gt", MANY)
+def test_many_tokens(E, k, G, tg, gt, score, biased, renormalize):
+    rng = np.random.default_rng([E, k, G, biased, 1])
+    bias = rng.standard_normal(E) * 0.1 if biased else None
+    for dtype, T in (("f32", 1027), ("bf16", 1025), ("f16", 1030)):
+        _check(rng.standard_normal((T, E)) * 1.5, k, dtype, bias, score=score, renormalize=renormalize, groups=G, topk_groups=tg,
+               group_top=gt, scale=2.5)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [(1, 1, 1), (4, 2, 2), (8, 3, 1)])
+def test_many_tokens_with_keys_closer_than_fp32_tells_apart(score, groups):
+    G, tg, gt = groups
+    rng = np.random.default_rng(6)
+    T, E = 1024, 64
+    for gap in (1e-9, 1e-7, 1e-6, 4e-6):
+        bias = (rng.standard_normal(E) * 0.05).astype(np.float32)
+        p = 0.3 + rng.permuted(np.tile(np.arange(E), (T, 1)), axis=1) * gap - bias.astype(np.float64)
+        logits = (np.log(p / (1 - p)) if score == "sigmoid" else np.log(p)).astype(np.float32)
+        _check(logits, 8, bias=bias, score=score, groups=G, topk_groups=tg, group_top=gt)
+        _check(logits, 7, score=score, groups=G, topk_groups=tg, group_top=gt)       # the logits themselves
+
+
+def _undecided(x, score, bias, groups, topk_groups, group_top):
+    """Tokens whose choice hangs on the last bits of 64-bit arithmetic: two groups (one in, one out) or two
+    experts of which different logits and biases make sums that are equal to 2^-46.  (Equal logits with equal
+    biases are a tie in any arithmetic, and decided.)  A score is off by at most 2 ulp of its exponential, the
+    sum of up to 96 terms and a quotient, and its sums with biases of magnitude < 2 by 2^-52 each: less than
+    110 x 2^-53 < 2^-46."""
+    near, out = 2.0 ** -46, np.zeros(len(x), bool)
+    b = np.zeros(x.shape[1]) if bias is None else bias
+    key = R.scores(x, score) + b
+    E = x.shape[1]
+    for t in range(len(x)):
+        allowed = np.ones(E, bool)
+        if topk_groups < groups:
+            order = np.argsort(-key[t].reshape(groups, -1), axis=1, kind="stable")[:, :group_top] + np.arange(groups)[:, None] * (E // groups)
+            strength = key[t][order].sum(axis=1)
+            what = [sorted(zip(x[t, o], b[o])) for o in order]
+            kept = set(np.argsort(-strength, kind="stable")[:topk_groups].tolist())
+            for g in kept:
+                for h in set(range(groups)) - kept:
+                    out[t] |= abs(strength[g] - strength[h]) <= near and what[g] != what[h]
+            allowed = np.isin(np.arange(E) // (E // groups), list(kept))
+        at = np.flatnonzero(allowed)
+        at = at[np.argsort(-key[t, at], kind="stable")]
+        gap = key[t, at][:-1] - key[t, at][1:]
+        differ = (x[t, at][:-1] != x[t, at][1:]) | (b[at][:-1] != b[at][1:])
+        out[t] |= bool(((gap <= near) & differ).any())
+    return out
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [(1, 1, 1), (8, 3, 1), (8, 3, 2), (2, 1, 2)])
+def test_many_tokens_with_ties_and_zeros(score, groups):
+    G, tg, gt = groups
+    rng = np.random.default_rng(7)
+    x = np.round(rng.standard_normal((1500, 96)) * 2) / 2     # few different values: ties within and across lanes
+    x[0:40] = 0.0
+    x[40:80, ::3] = -0.0                                      # equal to 0
+    x[80:90] = 88.0
+    x[90:100] = -200.0
+    for dtype in DT:
+        for bias in (None, np.zeros(96), np.round(rng.standard_normal(96)) / 4):
+            if bias is None and (gt == 1 or G == 1):      # the logits decide
+                _check(x, 8, dtype, bias, score=score, groups=G, topk_groups=tg, group_top=gt)
+                continue
+            seen, ids, w = _run(x, 8, dtype, bias, score=score, groups=G, topk_groups=tg, group_top=gt)
+            want, want_w = R.route(seen, 8, score, bias, groups=G, topk_groups=tg, group_top=gt)
+            sure = ~_undecided(seen, score, bias, G, tg, gt)
+            assert sure.sum() > 1350
+            assert np.array_equal(ids.cpu().numpy()[sure], want[sure])
+            assert (np.abs(w.cpu().numpy() - want_w) <= W_TOL * want_w + 2.0 ** -126)[sure].all()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [(1, 1, 1), (8, 3, 1), (8, 4, 2)])
+@pytest.mark.parametrize("kind", ["far", "masked", "lowest", "both ends", "few left", "none left", "inf", "offset"])
+def test_many_tokens_with_wide_biases(kind, groups, score):
+    """Biases that span more than the scores do, masks made of biases, biases that bar."""
+    G, tg, gt = groups
+    rng = np.random.default_rng(8)
+    E = 96
+    bias = (rng.standard_normal(E) * 0.1).astype(np.float32)
+    if kind == "far":
+        bias *= 100
+    elif kind == "masked":
+        bias[rng.permutation(E)[:80]] = -1e9
+    elif kind == "lowest":
+        bias[rng.permutation(E)[:90]] = np.finfo(np.float32).min
+    elif kind == "both ends":
+        bias[::2] = np.finfo(np.float32).min
+        bias[1::24] = np.finfo(np.float32).max
+    elif kind == "few left":
+        bias[5:] = -np.inf
+    elif kind == "none left":
+        bias[:] = np.where(np.arange(E) % 2, -np.inf, np.nan)
+    elif kind == "inf":
+        bias[[3, 50, 51]] = np.inf
+    elif kind == "offset":
+        bias += 1000.0
+    _check(rng.standard_normal((1024, E)) * 1.5, 8, "f32", bias, score=score, groups=G, topk_groups=tg, group_top=gt)
+
+
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("score,biased", list(itertools.product(["softmax", "sigmoid"], [False, True])))
+def test_many_tokens_with_barred_and_infinite_logits(score, biased, renormalize):
+    rng = np.random.default_rng(9)
+    T, E = 1100, 96
+    x = rng.standard_normal((T, E))
+    x[:900:9] = -np.inf
+    x[1:900:9] = np.nan
+    x[2:900:9, 1:] = -np.inf
+    x[3:900:9, :90] = -np.inf
+    x[4:900:9, 5:] = np.nan
+    x[5:900:9] = np.finfo(np.float32).min
+    x[6:900:9, ::2] = np.finfo(np.float32).min
+    x[7:900:9] = 1e4
+    x[8:900:9, 3] = 1e30
+    x[1000:1020, [7, 60]] = np.inf
+    bias = rng.standard_normal(E) * 0.1 if biased else None
+    for kw in (dict(), dict(groups=8, topk_groups=3, group_top=1), dict(groups=8, topk_groups=3, group_top=2)):
+        _check(x, 7, "f32", bias, score=score, renormalize=renormalize, **kw)
+
+
+@pytest.mark.parametrize("T", [20, 1040])
+def test_sigmoids_that_vanish_in_32_bits(T):
+    """Their ratios do not; those that vanish in 64 bits too leave nothing to divide."""
+    rng = np.random.default_rng(10)
+    x = np.round(rng.standard_normal((T, 64)) * 2)
+    x -= np.array([60, 64, 65, 90, 104, 200, 650, 700])[np.arange(T) % 8, None]
+    _check(x, 6, score="sigmoid")
+    _check(x, 6, score="sigmoid", groups=8, topk_groups=3, group_top=1)
+    _check(np.full((T, 64), -710.0), 6, score="sigmoid")
+
+
+def test_a_token_routes_alike_alone_and_among_many():
+    from mosaicist_b200 import ops
+
+    x = torch.randn(2000, 256, device="cuda")
+    bias = torch.randn(256, device="cuda") * 0.1
+    kw = dict(bias=bias, score="sigmoid", groups=8, topk_groups=4, group_top=2)
+    ids, w = ops.moe_route(x, 8, **kw)
+    for t in (0, 3, 1024, 1999):
+        one, ow = ops.moe_route(x[t:t + 1], 8, **kw)
+        assert torch.equal(one[0], ids[t]) and torch.allclose(ow[0], w[t], rtol=8 * 2.0 ** -24, atol=0)   # (the sum's order)
+
+
+def test_backward_with_a_tiny_scale():
+    """The quotient by the scale is one even where its reciprocal is not a number."""
+    from mosaicist_b200 import ops
+
+    scale = 1e-39
+    x = torch.randn(3, 16, device="cuda")
+    ids, w = ops.moe_route(x, 4, scale=scale)
+    g = torch.randn(3, 4, device="cuda")
+    dx = ops.moe_route_backward(g, x, ids, w, scale=scale)
+    assert torch.isfinite(dx).all() and float(dx.abs().max()) <= 8 * scale
