@@ -296,7 +296,7 @@ int msc_grouped_gemm_bf16_int4_ragged(const void* a, const void* b_q, const void
 /* x (rows, k), or with silu (rows, 2k) gate | up of which silu(gate) * up is taken in fp32 -> q (rows, k)
  * bytes, sf (ceil(k / 128), pitch) f32 with pitch = rows rounded up to 4; the columns behind `rows`
  * become 0.  With group_offsets / group_rows (l) only rows inside a group are read and written; groups
- * may start anywhere.  rows <= 524280; rows = 0 does nothing. */
+ * may start anywhere.  rows = 0 does nothing. */
 int msc_fp8_block_quantize(const void* x, int x_dtype, int silu, const int32_t* group_offsets,
                            const int32_t* group_rows, void* q, float* sf, int l, int rows, int k, void* stream);
 

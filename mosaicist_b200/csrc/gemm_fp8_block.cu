@@ -578,7 +578,7 @@ static int gemm_fp8_block(const void* a_q, const float* a_sf, const void* b_q, c
     return fail(MSC_ERR_BAD_ARG, "b_sf and row_scale must be 4-byte aligned");
   // tile coordinates are 32 bits
   if ((long long)l * n > 0x7fffff00LL) return fail(MSC_ERR_UNSUPPORTED, "l * n = %lld weight rows are too many", (long long)l * n);
-  if (rows_total > 0x7ffffe00) return fail(MSC_ERR_UNSUPPORTED, "rows=%d are too many", rows_total);
+  if (rows_total > 0x7ffffe00 || k > 0x7ffffe00) return fail(MSC_ERR_UNSUPPORTED, "rows=%d or k=%d is too large", rows_total, k);
   const long long ntiles = (n + 255) / 256;
   const long long max_tiles = ((long long)rows_total / 256 + (group_rows ? 2LL * l : 1LL)) * ntiles;
   if (max_tiles > 0x7fff0000LL) return fail(MSC_ERR_UNSUPPORTED, "the problem has too many tiles");

@@ -18,6 +18,7 @@
 
 namespace msc {
 
+constexpr int kMostOfASize = 0x7ffffe00;   // rounding a size up to a tile's stays within 32 bits
 constexpr float kFp8Max = 448.0f;
 constexpr float kLeastScale = 1.17549435e-38f;   // 2^-126
 
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const RowBlockPa
   __shared__ unsigned s_live;
   constexpr int kVecs = 16 / Vec16<T>::kPer;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int row0 = blockIdx.y * 8, row = row0 + warp;
+  const int row0 = blockIdx.x * 8, row = row0 + warp;
 
   // the rows of the tile that take part: all of them, or those that some group owns
   unsigned live = row0 + 8 <= p.rows ? 0xffu : (1u << max(p.rows - row0, 0)) - 1u;
@@ -152,8 +153,8 @@ __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const RowBlockPa
     }
   };
   const int pieces = (p.k + 511) >> 9;
-  load(blockIdx.x);
-  for (int c = blockIdx.x, buf = 0; c < pieces; c += gridDim.x, buf ^= 1) {
+  load(blockIdx.y);
+  for (int c = blockIdx.y, buf = 0; c < pieces; c += gridDim.y, buf ^= 1) {
     float v[16], amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const RowBlockPa
       for (int i = 0; i < 16; ++i) v[i] = silu_mul(v[i], up[i]);
       amax = amax_f32x16(v);
     }
-    if (c + (int)gridDim.x < pieces) load(c + gridDim.x);
+    if (c + (int)gridDim.y < pieces) load(c + gridDim.y);
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     const float s = block_scale(amax);
@@ -317,8 +318,8 @@ static int launch_rows(const RowBlockParams& p, bool silu, cudaStream_t stream) 
   const int tiles = (p.rows + 7) / 8, pieces = (p.k + 511) / 512;
   const int split = std::max(1, std::min(pieces, (16 * sms + tiles - 1) / tiles));
   cudaLaunchAttribute attr[1];
-  cudaLaunchConfig_t lc = pdl_launch_config(split, 256, 0, stream, attr);
-  lc.gridDim.y = (unsigned)tiles;
+  cudaLaunchConfig_t lc = pdl_launch_config(tiles, 256, 0, stream, attr);
+  lc.gridDim.y = (unsigned)split;
   auto kern = silu ? quantize_fp8_rows_kernel<T, true> : quantize_fp8_rows_kernel<T, false>;
   MSC_CUDA_OK(cudaLaunchKernelEx(&lc, kern, p));
   return MSC_OK;
@@ -339,7 +340,7 @@ int msc_fp8_block_quantize(const void* x, int x_dtype, int silu, const int32_t* 
   if (x_dtype < 0 || x_dtype > 2) return fail(MSC_ERR_UNSUPPORTED, "x_dtype must be 0 (bf16), 1 (f32) or 2 (f16), got %d", x_dtype);
   if (reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(sf) % 4)
     return fail(MSC_ERR_BAD_ARG, "x and q must be 16-byte aligned, sf 4-byte aligned");
-  if (rows > 65535 * 8) return fail(MSC_ERR_UNSUPPORTED, "rows=%d exceeds %d", rows, 65535 * 8);
+  if (rows > kMostOfASize || k > kMostOfASize) return fail(MSC_ERR_UNSUPPORTED, "rows=%d or k=%d exceeds %d", rows, k, kMostOfASize);
   if (rows == 0) return MSC_OK;
   RowBlockParams p;
   p.x = x; p.q = static_cast<uint8_t*>(q); p.sf = sf;
@@ -359,7 +360,8 @@ int msc_moe_permute_quantize_fp8_block(const void* tokens_bf16, const int32_t* i
     return fail(MSC_ERR_BAD_ARG, "NULL pointer");
   if (tokens < 0 || topk <= 0 || experts_local <= 0 || rows_cap <= 0)
     return fail(MSC_ERR_BAD_ARG, "tokens must not be negative, topk, experts_local and rows_cap must be positive");
-  if (hidden <= 0 || hidden % 16) return fail(MSC_ERR_BAD_ARG, "hidden=%d must be a positive multiple of 16", hidden);
+  if (rows_cap > kMostOfASize) return fail(MSC_ERR_UNSUPPORTED, "rows_cap=%d exceeds %d", rows_cap, kMostOfASize);
+  if (hidden <= 0 || hidden % 16 || hidden > 200 * 1024) return fail(MSC_ERR_BAD_ARG, "hidden=%d must be a positive multiple of 16, two rows of which fit in shared memory", hidden);
   if (topk > kFp8MaxTopk) return fail(MSC_ERR_UNSUPPORTED, "topk=%d exceeds %d", topk, kFp8MaxTopk);
   if (reinterpret_cast<uintptr_t>(tokens_bf16) % 16 || reinterpret_cast<uintptr_t>(a_q) % 16)
     return fail(MSC_ERR_BAD_ARG, "tokens and a_q must be 16-byte aligned");
@@ -394,6 +396,7 @@ int msc_fp8_block_quantize_weight(const void* w, int w_dtype, void* q, float* sf
   if (!w || !q || !sf) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
   if (l <= 0 || n <= 0 || k <= 0) return fail(MSC_ERR_BAD_ARG, "sizes must be positive");
   if (k % 16) return fail(MSC_ERR_BAD_ARG, "k=%d must be a multiple of 16", k);
+  if (n > kMostOfASize || k > kMostOfASize) return fail(MSC_ERR_UNSUPPORTED, "n=%d or k=%d exceeds %d", n, k, kMostOfASize);
   if (w_dtype < 0 || w_dtype > 2) return fail(MSC_ERR_UNSUPPORTED, "w_dtype must be 0 (bf16), 1 (f32) or 2 (f16), got %d", w_dtype);
   if (reinterpret_cast<uintptr_t>(w) % 16 || reinterpret_cast<uintptr_t>(q) % 16 || reinterpret_cast<uintptr_t>(sf) % 4)
     return fail(MSC_ERR_BAD_ARG, "w and q must be 16-byte aligned, sf 4-byte aligned");

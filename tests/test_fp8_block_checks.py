@@ -151,7 +151,7 @@ def test_route_backward_refusals(lib, args):
     (P, 0, 0, P, None, P, P, 1, 8, 128), (P, 0, 0, None, P, P, P, 1, 8, 128), (P, 0, 0, P, P, P, P, 0, 8, 128), (P, 0, 0, None, None, P, P, 0, -1, 128),
     (P, 0, 0, None, None, P, P, 0, 8, 0), (P, 0, 0, None, None, P, P, 0, 8, 120), (P, 3, 0, None, None, P, P, 0, 8, 128),
     (P + 8, 0, 0, None, None, P, P, 0, 8, 128), (P, 0, 0, None, None, P + 8, P, 0, 8, 128), (P, 0, 0, None, None, P, P + 2, 0, 8, 128),
-    (P, 0, 0, None, None, P, P, 0, 600000, 128)])
+    (P, 0, 0, None, None, P, P, 0, 0x7fffffff, 128), (P, 0, 0, None, None, P, P, 0, 8, 0x7ffffff0)])
 def test_quantizer_refusals(lib, args):
     assert lib.msc_fp8_block_quantize(*args, None) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
 
@@ -159,7 +159,7 @@ def test_quantizer_refusals(lib, args):
 @pytest.mark.parametrize("args", [
     (None, 0, P, P, 1, 128, 128), (P, 0, None, P, 1, 128, 128), (P, 0, P, None, 1, 128, 128), (P, 0, P, P, 0, 128, 128), (P, 0, P, P, 1, 0, 128),
     (P, 0, P, P, 1, 128, 0), (P, 0, P, P, 1, 128, 100), (P, 7, P, P, 1, 128, 128), (P + 4, 0, P, P, 1, 128, 128), (P, 0, P + 4, P, 1, 128, 128),
-    (P, 0, P, P + 1, 1, 128, 128), (P, 0, P, P, 70000, 128, 128)])
+    (P, 0, P, P + 1, 1, 128, 128), (P, 0, P, P, 70000, 128, 128), (P, 0, P, P, 1, 0x7fffffff, 128), (P, 0, P, P, 1, 128, 0x7ffffff0)])
 def test_weight_quantizer_refusals(lib, args):
     assert lib.msc_fp8_block_quantize_weight(*args, None) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
 
@@ -169,7 +169,8 @@ def test_weight_quantizer_refusals(lib, args):
     (P, P, P, None, P, 0, 8, 128, 128, 0), (P, P, P, P, None, 0, 8, 128, 128, 0), (P, P, P, P, P, 3, 8, 128, 128, 0),
     (P, P, P, P, P, 0, -1, 128, 128, 0), (P, P, P, P, P, 0, 8, 0, 128, 0), (P, P, P, P, P, 0, 8, 128, 0, 0), (P, P, P, P, P, 0, 8, 100, 128, 0),
     (P, P, P, P, P, 0, 8, 128, 100, 0), (P, P, P, P, P, 0, 8, 128, 128, -2), (P + 8, P, P, P, P, 0, 8, 128, 128, 0), (P, P + 4, P, P, P, 0, 8, 128, 128, 0),
-    (P, P, P + 1, P, P, 0, 8, 128, 128, 0), (P, P, P, P + 2, P, 0, 8, 128, 128, 0), (P, P, P, P, P + 8, 0, 8, 128, 128, 0)])
+    (P, P, P + 1, P, P, 0, 8, 128, 128, 0), (P, P, P, P + 2, P, 0, 8, 128, 128, 0), (P, P, P, P, P + 8, 0, 8, 128, 128, 0),
+    (P, P, P, P, P, 0, 0x7fffffff, 128, 128, 0), (P, P, P, P, P, 0, 8, 0x7ffffff8, 128, 0), (P, P, P, P, P, 0, 8, 128, 0x7ffffff0, 0)])
 def test_product_refusals(lib, args):
     assert lib.msc_gemm_fp8_block(*args, None) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
 
@@ -199,7 +200,7 @@ def test_operators_can_be_traced(fake):
 @pytest.mark.parametrize("kw", [
     dict(tokens_ptr=None), dict(ids=None), dict(w=None), dict(rank=None), dict(offs=None), dict(a_q=None), dict(a_sf=None), dict(rw=None), dict(rt=None),
     dict(tokens=-1), dict(hidden=0), dict(hidden=100), dict(topk=0), dict(topk=65), dict(local=0), dict(cap=0), dict(tokens_ptr=P + 2), dict(a_q=P + 8),
-    dict(a_sf=P + 2), dict(ids=P + 1), dict(hidden=200000)])
+    dict(a_sf=P + 2), dict(ids=P + 1), dict(hidden=200000), dict(hidden=0x7ffffff0), dict(cap=0x7fffffff)])
 def test_dispatch_refusals(lib, kw):
     a = dict(tokens_ptr=P, ids=P, w=P, rank=P, offs=P, tokens=8, hidden=256, topk=2, first=0, local=4, a_q=P, a_sf=P, rw=P, rt=P, cap=512) | kw
     assert lib.msc_moe_permute_quantize_fp8_block(*a.values(), None) in (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)

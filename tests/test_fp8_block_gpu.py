@@ -48,6 +48,19 @@ def test_quantize_rows(rows, k, dtype):
     assert np.array_equal(q.cpu().numpy(), want_q)
 
 
+def test_quantize_more_rows_than_a_grid_is_high():
+    """The rows of 65536 tokens with 8 experts each, and a few."""
+    rows, k = 65536 * 8 + 3, 32
+    from mosaicist_b200 import ops
+
+    x = torch.randn(rows, k, device="cuda", dtype=torch.bfloat16)
+    q, sf = ops.quantize_fp8_block(x)
+    part, part_sf = ops.quantize_fp8_block(x[-4:].contiguous())
+    assert torch.equal(q[-4:].view(torch.uint8), part.view(torch.uint8)) and torch.equal(sf[:, rows - 4:rows], part_sf)
+    assert float(sf[:, rows:].abs().sum()) == 0
+    assert torch.equal(sf[0, :rows], (x.float().abs().amax(1).cpu() / 448.0).cuda())
+
+
 @pytest.mark.parametrize("dtype", DT)
 @pytest.mark.parametrize("shape", [(8, 16), (1, 128), (128, 128), (129, 144), (1048, 400), (3, 260, 272)])
 def test_quantize_weight(shape, dtype):
