@@ -15,11 +15,20 @@
 // Tiles of up to 64 tokens (a decode step, what is left over of a group) exchange the roles: 256 weight rows
 // are the M side and the tokens N, rounded up to 32, so that a tile costs little more than its weights'
 // way into shared memory.  A lane then is a weight row and a register a token; the tokens' scales come by shuffle.
+// (64 groups of 48 tokens, 4096 x 2048: 135 us, 147 with tokens on M; of 64 tokens 139 against 150.)
 //
 // A dense product with fewer tiles than half the chip has CTA pairs is split along K: clusters of two or
 // four pairs take a tile, leave their sums in shared memory and each adds up its share of the columns, in the order
 // of K.  And where the last round of a dense product's tiles would keep only a few pairs busy, its tiles are
 // taken in quarters of 64 tokens.
+//
+// What bounds it.  Large products: the consumers.  The MMAs of a K block take 513 cycles, reading 256 columns out of
+// tensor memory, adding them and handing them back about 750, so 8192 x 8192 x 7168 runs in 405 to 417 us, 2.3
+// PFLOP/s, about 70 % of twice the measured bf16 rate (the MX kernel, whose scales the tensor core applies, 307 us).
+// Wider or more consumer groups do not fit the registers, scales from a ring in shared memory cost more of its bandwidth
+// than they save (490 us), and accumulators of 128 columns in turn double the hand-overs.  Few tokens: the weights'
+// traffic (64 groups of 0 to 16 rows, 4096 x 7168: 330 us, 5.5 TB/s) or, for one small matrix, the launch
+// and the ring's first fill (16 x 7168 x 2048: 10 us).
 #include "gemm_common.cuh"
 #include "quantize_common.cuh"
 
@@ -608,14 +617,16 @@ static int gemm_fp8_block(const void* a_q, const float* a_sf, const void* b_q, c
   long long units = max_tiles;                 // tiles, or clusters' pairs
   if (!group_rows) {
     const long long tiles = ((long long)rows_total + 255) / 256 * ntiles;
-    const int rest = rows_total % 256;
-    const long long whole = rest >= 1 && rest <= Fp8Smem::kFewTokens ? tiles - ntiles : tiles;   // more than 64 tokens
-    const long long done = tiles / room * room;
+    const long long done = tiles / room * room;   // in full rounds
     units = tiles;
-    while (p.splits < 4 && tiles * p.splits * 2 <= room && p.kblocks >= 8 * p.splits) p.splits *= 2;
+    // A share of K has 12 blocks at least: the sums' way through shared memory costs what a few blocks do
+    // (64 x 2048 x 7168, four shares of 14: 22.6 us against 30.7; 16 x 7168 x 2048, two of 8: 18.4 against 16.4).
+    while (p.splits < 4 && tiles * p.splits * 2 <= room && p.kblocks >= 24 * p.splits) p.splits *= 2;
     if (p.splits > 1) {
       units = tiles * p.splits;
-    } else if (whole > done && 4 * (whole - done) + (tiles - whole) <= room) {
+    } else if (tiles > done && 4 * (tiles - done) <= room) {
+      // A quarter to a pair (1024 x 5120 x 4096, 6 tiles in 24 quarters: 41.0 us against 45.1); where pairs would take
+      // two of them nothing is gained (4101 x 7168 x 4096, 32 tiles: 133 us against 125).
       p.quarters_from = (int)done;
       units = done + 4 * (tiles - done);
     }

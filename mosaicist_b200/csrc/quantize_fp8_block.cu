@@ -265,7 +265,8 @@ __global__ void __launch_bounds__(512) moe_permute_quantize_fp8_kernel(const Fp8
 
 // ---- weights -------------------------------------------------------------------------------
 // A CTA per 128 x 128 block, whose values stay in registers between the maximum and the quotients: a
-// thread holds 64 of them in four row pieces of 16.
+// thread holds 64 of them in four row pieces of 16.  Four CTAs an SM keep enough loads in flight: 16 x 4096 x 7168 bf16
+// in 240 us, 5.9 TB/s of read and written bytes, 259 us with two; fp32 values take twice the registers and two CTAs.
 struct WeightBlockParams {
   const void* w;    // (l, n, k)
   uint8_t* q;       // (l, n, k)
@@ -316,7 +317,9 @@ template <class T>
 static int launch_rows(const RowBlockParams& p, bool silu, cudaStream_t stream) {
   const int sms = num_sms();
   if (sms <= 0) return fail(MSC_ERR_CUDA, "could not query the SM count");
-  // as many CTAs per row as it takes to give every SM sixteen
+  // As many CTAs per row as it takes to give every SM sixteen, of which eight are resident: with up to 64 the pieces of
+  // many rows lose their loads in flight (gate | up of 64 groups 52 us against 36), with 4 a middling number
+  // of rows fills the SMs badly (4096 x 2048 9.7 us against 8.4).
   const int tiles = (p.rows + 7) / 8, pieces = (p.k + 511) / 512;
   const int split = std::max(1, std::min(pieces, (16 * sms + tiles - 1) / tiles));
   cudaLaunchAttribute attr[1];

@@ -253,6 +253,20 @@ def test_last_round_in_quarter_tiles(m, n, k, ctas):
     assert (out[m:] == 3).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 264, 4112), (33, 1000, 4112), (64, 8, 6160), (200, 520, 7184), (300, 1304, 4112), (257, 256, 16400)])
+def test_few_tiles_split_along_k(m, n, k):
+    """Two and four shares of K, uneven ones too, of tiles of either kind."""
+    from mosaicist_b200 import ops
+
+    rng = np.random.default_rng([m, n, k])
+    a, sa, b, sb = _operands(rng, m, 1, n, k, True)
+    want = F.product(a, sa, b[0], sb[0])[0]
+    out = torch.full((m + 9, n), 3.0, dtype=torch.float32, device="cuda")
+    got = ops.gemm_fp8_block(T(a), _dev_sf(sa), T(b[0]), T(sb[0]), out=out[:m])
+    _check(got, want, None, k, "f32", True)
+    assert (out[m:] == 3).all()
+
+
 def test_dense_writes_its_rows_only():
     from mosaicist_b200 import ops
 
