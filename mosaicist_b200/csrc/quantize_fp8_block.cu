@@ -114,8 +114,9 @@ struct RowBlockParams {
 // A CTA takes 8 rows, a warp one of them, and walks its share of the row's pieces of 512 columns with the next
 // piece's loads in flight; a thread holds 16 values, 8 lanes share a block.  The 32 scales of a
 // piece meet in shared memory and leave as 32-byte stretches of the column layout.
-// Measured: gate | up of 15361 rows x 2048 bf16 in 64 groups with silu, 161 MB moved in 34 us, 4.7 TB/s (silu is
-// four instructions and two of the special unit per value); 16 rows x 7168 in 4.3 us, which is the launch.
+// Measured: gate | up of 16300 rows x 2048 bf16 in 64 groups with silu, 167 MB moved in 36 us, 4.6 TB/s (silu and its
+// two special functions a value keep it below the 5.2 TB/s of 16384 x 7168 without); 16 rows x 7168 in 4.4 us, which is
+// the launch.
 template <class T, bool SILU>
 __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const RowBlockParams p) {
   grid_dependency_wait();
