@@ -16,12 +16,12 @@
 // Two layouts.  A warp per token, the experts of a group spread over the lanes, 32 to a register slot: a group's
 // maximum is one warp reduction (redux.sync) per slot, and a thread-wide maximum over the slots, one reduction and
 // one minimum over the experts that hold it make a choice.  That is the shortest way for a few tokens and serves up
-// to 1024 experts, but 256 experts, top 8 of 4 of 8 groups take about 1330 instructions per token, most of
+// to 1024 experts, but 256 experts, top 8 of 4 of 8 groups take about 1330 instructions per token (533 by eight lanes), most of
 // them the serial rounds of choosing.  From 1024 tokens on, and up to 256 experts, eight lanes per token share
 // these rounds among four tokens (below).
 //
 // Neither is bound by memory: 8192 tokens of 256 fp32 logits are 8.9 MB, 1.4 us, and take 12 us with sigmoid,
-// bias and 4 of 8 groups (21 a warp per token), 5 us for 128 bf16 experts without them; 16 tokens take 4.5 us. What is left
+// bias and 4 of 8 groups (21 a warp per token), 5 us for 128 bf16 experts without them; 16 tokens take 4 to 5.5 us. What is left
 // is the chain of one warp's steps (3 to 4 us) and, where keys lie close, the tokens that are looked at in 64 bits.
 //
 // A logit of -inf or NaN, or a bias of -inf or NaN, bars its expert.  Where fewer than topk experts are
