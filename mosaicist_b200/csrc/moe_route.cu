@@ -657,8 +657,10 @@ __global__ void __launch_bounds__(32 * kOctetWarps) moe_route_octets_kernel(cons
         const int slot = quad * (PER / 4) + i;
         const float x = s_x[q * kTokenPitch + sub * kPitch + slot];
         float v = x;
-        if (KEYS != kByLogit && x != -INFINITY)
-          v = fmaxf(fmaf(sigmoid(x) + s_bias[warp][sub * kPitch + slot], unit, end), 0x1p23f + 1.0f) - 0x1p24f;
+        if (KEYS != kByLogit && x != -INFINITY) {
+          v = fmaf(sigmoid(x) + s_bias[warp][sub * kPitch + slot], unit, end);
+          if (v != -INFINITY) v = fmaxf(v, 0x1p23f + 1.0f) - 0x1p24f;   // (a barred expert's is not lifted into the window)
+        }
         const uint32_t who = __ballot_sync(0xffffffffu, in && v >= cut);
         const int place = n + __popc(who & ((1u << lane) - 1u));
         if (in && v >= cut && place < 32) s_some[warp][place] = e0 + slot;

@@ -443,3 +443,24 @@ def test_backward_with_a_tiny_scale():
     g = torch.randn(3, 4, device="cuda")
     dx = ops.moe_route_backward(g, x, ids, w, scale=scale)
     assert torch.isfinite(dx).all() and float(dx.abs().max()) <= 8 * scale
+
+
+@pytest.mark.parametrize("masks", [0, 10])
+@pytest.mark.parametrize("groups", [(1, 1, 1), (2, 2, 1), (4, 3, 1), (4, 3, 2)])
+@pytest.mark.parametrize("E", [16, 32])
+def test_many_tokens_with_close_keys_beside_barred_biases(E, groups, masks):
+    """Sigmoids that fall together at the lower end of the keys' window, so that every expert comes into question and
+    is ranked in 64 bits, but for those that a NaN or -inf bias bars."""
+    G, tg, gt = groups
+    rng = np.random.default_rng([E, G, gt, masks])
+    T = 1025
+    bias = np.zeros(E, np.float32)
+    at = rng.permutation(E)
+    bias[at[2:2 + masks]] = -1e9
+    bias[at[0]], bias[at[1]] = np.nan, -np.inf
+    for far in (-30.0, 0.0):
+        x = rng.standard_normal((T, E)) + far
+        _, ids, w = _check(x, 8 if G == 1 else 6, "f32", bias, score="sigmoid", groups=G, topk_groups=tg, group_top=gt)
+        got = ids.cpu().numpy()
+        assert not np.isin(got, at[:2]).any()
+        assert all(len(set(r)) == len(r) for r in got.tolist())
