@@ -93,10 +93,30 @@ class TokenExchange:
         return back, position.to(torch.int32)
 
 
+def _route(layer, logits, experts_total: int, topk: int, ids, weights) -> None:
+    """Routes logits (T, experts_total) by the rule of `layer`, which holds a share of the experts, into ids and
+    weights (T, topk): by its RouteConfig and bias, or by the plain rule where it has none."""
+    config = getattr(layer, "route_config", None)
+    if config is None:
+        from . import _lib
+
+        _lib.check(_lib.load().msc_moe_route_topk(logits.data_ptr(), ids.data_ptr(), weights.data_ptr(), logits.shape[0],
+                                                  logits.shape[1], topk, torch.cuda.current_stream().cuda_stream))
+        return
+    from . import ops
+
+    if logits.shape[1] != experts_total:
+        raise ValueError(f"logits of {logits.shape[1]} experts, the layers have {experts_total}")
+    ops.moe_route(logits, topk, config.score, layer.route_bias, config.groups, config.topk_groups, config.group_top,
+                  config.renormalize, config.scale, (ids, weights))
+
+
 class ExpertParallelMoE:
-    """MegaMoE over expert-parallel ranks.  `layer` is this rank's `moe.MegaMoE` holding its
-    local experts, built with topk=1, expert_first=rank*E_local and max_tokens >= the most
-    rows a rank can receive."""
+    """MegaMoE over expert-parallel ranks.  `layer` is this rank's `moe.MegaMoE` or
+    `moe.MegaMoEFp8Block` holding its local experts, built with topk=1,
+    expert_first=rank*E_local and max_tokens >= the most rows a rank can receive.  Its
+    RouteConfig and bias (over all experts), if it has them, are the rule that `topk` experts
+    are chosen by here."""
 
     def __init__(self, layer, experts_total: int, topk: int, group=None):
         self.layer, self.topk = layer, topk
@@ -106,7 +126,8 @@ class ExpertParallelMoE:
         self._zero = torch.zeros((1,), dtype=torch.int32, device=layer.ids.device)
 
     def forward(self, tokens, logits):
-        """tokens (T_local, h) bf16, logits (T_local, experts_total) f32 -> (T_local, h) bf16.
+        """tokens (T_local, h) bf16, logits (T_local, experts_total) f32 (with a RouteConfig bf16 and f16
+        too) -> (T_local, h) bf16.
         The result is defined only while the library's status word stays 0 (`_lib.status_word()`):
         a step that overflowed a rank's rows_cap (bit 0x00E00000) drops the pairs that did not fit
         from the sum, one whose wait for a peer ran out (0x00D00000) computed on incomplete data."""
@@ -119,8 +140,7 @@ class ExpertParallelMoE:
         ids = torch.empty((T, k), dtype=torch.int32, device=dev)
         weights = torch.empty((T, k), dtype=torch.float32, device=dev)
         st = torch.cuda.current_stream().cuda_stream
-        _lib.check(lib.msc_moe_route_topk(logits.data_ptr(), ids.data_ptr(), weights.data_ptr(), T,
-                                          logits.shape[1], k, st))
+        _route(self.layer, logits, self.exchange.world * self.exchange.experts_local, k, ids, weights)
         rows, e_ids, w = self.exchange.dispatch(tokens, ids, weights)
         R = rows.shape[0]
         if R > self.layer.max_tokens:
@@ -251,7 +271,8 @@ class PeerExpertParallelMoE:
     """MegaMoE over expert-parallel ranks with dispatch and combine through peer memory.
 
     `layer` is this rank's `moe.MegaMoE` over its local experts, built with topk=1,
-    expert_first=rank * E_local, rows_cap=`rows_cap` and workspace=this rank's exchange buffers;
+    expert_first=rank * E_local, rows_cap=`rows_cap` and workspace=this rank's exchange buffers; its
+    RouteConfig and bias (over all experts), if it has them, are the rule that `topk` experts are chosen by;
     `pointers[name][r]` are the device addresses of rank r's a_q / sf_rows / row_weight / y
     (`PeerBuffers.pointers`), `sf_rows` this rank's own (rows_cap, h/16) scale rows; `input_gs_all` (experts_total,) f32 holds every expert's input
     global scale, since the sender quantises.  The phases `count`, `place`, `dispatch`,
@@ -276,6 +297,10 @@ class PeerExpertParallelMoE:
         counts the same way; without them `forward` uses an NCCL all-gather and two all-reduces."""
         import ctypes
 
+        from .moe import MegaMoEFp8Block
+
+        if isinstance(layer, MegaMoEFp8Block):
+            raise ValueError("the peer-memory exchange carries NVFP4 rows: the layer must be a MegaMoE")
         if experts_total % world:
             raise ValueError(f"{experts_total} experts do not split over {world} ranks")
         if layer.topk != 1 or layer.expert_first != rank * (experts_total // world):
@@ -348,8 +373,7 @@ class PeerExpertParallelMoE:
             raise ValueError(f"{T} tokens exceed the workspace built for {self.max_tokens}")
         self._T = T
         st = self._stream()
-        _lib.check(lib.msc_moe_route_topk(logits.data_ptr(), self.ids.data_ptr(), self.weights.data_ptr(),
-                                          T, logits.shape[1], self.topk, st))
+        _route(self.layer, logits, self.E, self.topk, self.ids[:T], self.weights[:T])
         _lib.check(lib.msc_moe_plan(self.ids.data_ptr(), T * self.topk, 0, self.E,
                                     self.rank_in_group.data_ptr(), self.counts.data_ptr(),
                                     self._tmp.data_ptr(), self._tmp[self.E:].data_ptr(),

@@ -250,3 +250,31 @@ def test_wait_without_signal_times_out_and_reports():
     assert _lib.status_word() & 0x00D00000
     assert int((flags + 1).sum()) == 64          # the device still answers
     assert _lib.status_word() == 0
+
+
+@pytest.mark.parametrize("push", [False, True], ids=["pull", "push"])
+def test_emulated_ranks_route_by_the_layers_rule(push):
+    from mosaicist_b200 import _lib, ops
+    from mosaicist_b200.moe import MegaMoE, RouteConfig
+
+    world, E, k, h, n, T_loc = 2, 32, 4, 256, 128, 60
+    w = _weights(E, h, n, seed=3)
+    rng = np.random.default_rng(4)
+    cfg = RouteConfig(score="sigmoid", groups=4, topk_groups=2, group_top=2, scale=2.0)
+    bias = T((0.2 * rng.standard_normal(E)).astype(np.float32))
+    gs, gs2 = np.full(E, 2688.0 / 5.0, np.float32), np.full(E, 2688.0 / 4.0, np.float32)
+    rows_cap = (world * T_loc * k + 127 * (E // world) + 127) // 128 * 128
+    ranks = _layers(world, E, k, h, n, T_loc, rows_cap, w, gs, gs2, push)
+    for ep in ranks:
+        ep.layer.route_config, ep.layer.route_bias = cfg, bias
+    tk = [T(rng.standard_normal((T_loc, h)).astype(np.float32)).to(torch.bfloat16) for _ in range(world)]
+    lg = [T(rng.standard_normal((T_loc, E)).astype(np.float32)) for _ in range(world)]
+    outs, _ = _lockstep(ranks, tk, lg)
+    d = _dev_weights(w)
+    single = MegaMoE(d["w1_q"], d["w1_sf"], d["w1_gs"], d["w1_alpha"], d["w2_q"], d["w2_sf"], d["w2_gs"], d["w2_alpha"],
+                     T(gs), T(gs2), topk=k, max_tokens=T_loc, route=cfg, route_bias=bias)
+    for r in range(world):
+        ids, _ = ops.moe_route(lg[r], k, "sigmoid", bias, 4, 2, 2, True, 2.0)
+        assert torch.equal(ranks[r].ids[:T_loc], ids)
+        assert torch.equal(outs[r], single.forward(tk[r], lg[r]))
+    assert _lib.status_word() == 0

@@ -187,3 +187,24 @@ def test_the_nvfp4_layer_takes_a_route_config():
     assert not torch.equal(plain.forward(x, logits), got)
     with pytest.raises(ValueError):
         routed.forward(x, logits[:-1])
+
+
+def test_one_expert_parallel_rank_equals_the_layer():
+    """ExpertParallelMoE of one rank over an FP8 layer with a router of its own: the layer's result, bit for bit."""
+    import torch.distributed as dist
+
+    from mosaicist_b200.moe import MegaMoEFp8Block, RouteConfig
+    from mosaicist_b200.parallel import ExpertParallelMoE
+
+    E, h, n, k, tokens = 8, 256, 128, 3, 50
+    w = [T(v) for v in _weights(E, h, n, 5)]
+    cfg = RouteConfig(score="sigmoid", groups=2, topk_groups=1, group_top=2, scale=2.5)
+    bias = torch.randn(E, device="cuda") * 0.2
+    x, logits = torch.randn(tokens, h, device="cuda").bfloat16(), torch.randn(tokens, E, device="cuda").bfloat16()
+    want = MegaMoEFp8Block(*w, topk=k, max_tokens=tokens, route=cfg, route_bias=bias).forward(x, logits)
+    dist.init_process_group("nccl", store=dist.HashStore(), rank=0, world_size=1, device_id=torch.device("cuda", 0))
+    try:
+        share = MegaMoEFp8Block(*w, topk=1, max_tokens=tokens * k, route=cfg, route_bias=bias)
+        assert torch.equal(ExpertParallelMoE(share, E, k).forward(x, logits), want)
+    finally:
+        dist.destroy_process_group()

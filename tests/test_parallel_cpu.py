@@ -144,3 +144,103 @@ def test_exchange_layout_sections_are_aligned_and_disjoint():
         assert spans[-1][0] + spans[-1][1] <= total
     with pytest.raises(ValueError):
         exchange_views(torch.zeros(10, dtype=torch.uint8), 128, 256)
+
+
+def _router(experts):
+    """A router's rule, a stand-in for the kernel that follows it, and a library that has no plain rule."""
+    import numpy as np
+
+    from mosaicist_b200.moe import RouteConfig
+    from oracle import route as R
+
+    cfg = RouteConfig(score="sigmoid", groups=2, topk_groups=1, group_top=2, scale=2.5)
+    bias = torch.from_numpy((0.2 * np.random.default_rng(1).standard_normal(experts)).astype(np.float32))
+
+    def moe_route(logits, topk, score, b, groups, topk_groups, group_top, renormalize, scale, out):
+        assert b is bias
+        ids, w = R.route(logits.numpy(), topk, score, b.numpy(), groups, topk_groups, group_top, renormalize, scale)
+        out[0].copy_(torch.from_numpy(ids))
+        out[1].copy_(torch.from_numpy(w.astype(np.float32)))
+        return out
+
+    class Library:
+        msc_moe_unpermute = msc_moe_plan = staticmethod(lambda *args: 0)
+
+        def msc_moe_route_topk(self, *args):
+            raise AssertionError("the plain rule in place of the layer's")
+
+    return cfg, bias, moe_route, Library()
+
+
+def _stand_in(cfg, bias, **kw):
+    from types import SimpleNamespace
+
+    return SimpleNamespace(**(dict(topk=1, expert_first=0, route_config=cfg, route_bias=bias, max_tokens=512,
+                                   ids=torch.full((512, 1), -1, dtype=torch.int32), weights=torch.zeros(512, 1)) | kw))
+
+
+def _routing_worker(rank, world, port, experts):
+    """Rows reach the experts that the layer's own router chooses, with its weights."""
+    from types import SimpleNamespace
+
+    from mosaicist_b200 import _lib, ops
+    from mosaicist_b200.parallel import ExpertParallelMoE
+    from oracle import route as R
+
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        cfg, bias, ops.moe_route, library = _router(experts)
+        _lib.load = lambda: library
+        torch.cuda.current_stream = lambda: SimpleNamespace(cuda_stream=0)
+        logits = [torch.randn(30 + r, experts, generator=torch.Generator().manual_seed(r)) for r in range(world)]
+        k, first = 3, rank * (experts // world)
+        layer = _stand_in(cfg, bias, expert_first=first, forward=lambda rows, none: rows)
+        ep = ExpertParallelMoE(layer, experts, k)
+        ep.forward(torch.zeros(30 + rank, 8), logits[rank])
+        want = []
+        for lg in logits:
+            ids, w = R.route(lg.numpy(), k, cfg.score, bias.numpy(), cfg.groups, cfg.topk_groups, cfg.group_top, cfg.renormalize, cfg.scale)
+            want += [(int(e), float(x)) for e, x in zip(ids.ravel(), w.astype("float32").ravel()) if first <= e < first + experts // world]
+        assert want and list(zip(layer.ids[:len(want), 0].tolist(), layer.weights[:len(want), 0].tolist())) == want
+        assert int(layer.ids[len(want)]) == -1
+        with pytest.raises(ValueError, match="experts"):
+            ep.forward(torch.zeros(30 + rank, 8), logits[rank][:, 1:])
+    finally:
+        dist.destroy_process_group()
+
+
+def test_expert_parallel_layers_route_by_the_layers_rule_world2():
+    mp.spawn(_routing_worker, args=(2, _free_port(), 8), nprocs=2, join=True)
+
+
+def test_peer_layers_route_by_the_layers_rule(monkeypatch):
+    import numpy as np
+
+    from types import SimpleNamespace
+
+    from mosaicist_b200 import _lib, ops
+    from mosaicist_b200.moe import MegaMoEFp8Block
+    from mosaicist_b200.parallel import PeerExpertParallelMoE
+    from oracle import route as R
+
+    experts, k, T = 8, 3, 20
+    cfg, bias, moe_route, library = _router(experts)
+    monkeypatch.setattr(ops, "moe_route", moe_route)
+    monkeypatch.setattr(_lib, "load", lambda: library)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: SimpleNamespace(cuda_stream=0))
+    sf_rows = torch.zeros(128, 4, dtype=torch.uint8)
+    pointers = dict(a_q=[0], sf_rows=[sf_rows.data_ptr()], row_weight=[0], y=[0])
+
+    def make(layer):
+        return PeerExpertParallelMoE(layer, pointers, sf_rows, torch.ones(experts), experts, k, T + 2, 0, 1)
+
+    ep = make(_stand_in(cfg, bias, rows_cap=128, h=64, a_q=torch.zeros(128, 32, dtype=torch.uint8)))
+    logits = torch.randn(T, experts, generator=torch.Generator().manual_seed(3))
+    ep.count(logits)
+    ids, w = R.route(logits.numpy(), k, cfg.score, bias.numpy(), cfg.groups, cfg.topk_groups, cfg.group_top, cfg.renormalize, cfg.scale)
+    assert np.array_equal(ep.ids[:T].numpy(), ids) and np.array_equal(ep.weights[:T].numpy(), w.astype(np.float32))
+    with pytest.raises(ValueError, match="experts"):
+        ep.count(logits[:, :-1])
+    with pytest.raises(ValueError, match="NVFP4"):         # the exchange has no room for rows of 8 bits
+        make(object.__new__(MegaMoEFp8Block))
