@@ -304,7 +304,8 @@ int msc_fp8_block_quantize(const void* x, int x_dtype, int silu, const int32_t* 
  * hidden) bf16), quantises it once and writes it at row group_offsets[e] + rank (msc_moe_plan) of a_q (rows_cap,
  * hidden) and a_sf (ceil(hidden / 128), rows_cap rounded up to 4), with the pair's routing weight in row_weight
  * (rows_cap) f32 and its token in row_token (rows_cap) i32.  hidden % 16 == 0, topk <= 64, a_q 16-byte
- * aligned; a row that would lie at or beyond rows_cap is left out.  tokens = 0 does nothing. */
+ * aligned; a row that would lie at or beyond rows_cap is left out, which raises bit 0x00E00000 in the
+ * status word.  tokens = 0 does nothing. */
 int msc_moe_permute_quantize_fp8_block(const void* tokens_bf16, const int32_t* ids, const float* weights,
                                        const int32_t* rank, const int32_t* group_offsets, int tokens, int hidden,
                                        int topk, int expert_first, int experts_local, void* a_q, float* a_sf,
@@ -401,8 +402,9 @@ int msc_moe_plan_noalloc(const int32_t* ids, int entries, int expert_first, int 
  * with its expert's global scale (arithmetic of quantize_nvfp4, nvfp4.py:39-57) and writes it
  * at row group_offsets[e] + rank: a_q (rows_cap, hidden/2), a_sf tiled
  * (rows_cap/128, hidden/64, 32, 16), plus row_weight (rows_cap) f32 = the pair's routing weight
- * and row_token (rows_cap) i32.  rows_cap is a multiple of 128 >= total_rows.  hidden % 64 == 0,
- * topk <= 64, a_q 16-byte aligned (rows leave shared memory as bulk copies).
+ * and row_token (rows_cap) i32.  rows_cap is a multiple of 128 >= total_rows; rows at or beyond it
+ * (without sf_rows 0 means no bound) are left out, which raises bit 0x00E00000 in the status word.
+ * hidden % 64 == 0, topk <= 64, a_q 16-byte aligned (rows leave shared memory as bulk copies).
  * sf_rows (rows_cap, hidden/16) u8 or NULL: staging for the scales.  With it (hidden % 256 == 0,
  * rows_cap a multiple of 128, both scale buffers 16-byte aligned) and tokens * topk > 4096 every
  * row's scale bytes leave as one bulk copy into sf_rows and a second kernel re-tiles them into
@@ -410,7 +412,7 @@ int msc_moe_plan_noalloc(const int32_t* ids, int entries, int expert_first, int 
  * (device, i32, or NULL) is the row count msc_moe_plan produced and bounds that pass, padding
  * rows inside it receive whatever sf_rows held.  For up to 4096 rows, where the second launch
  * costs more than it saves, and without sf_rows the tiling is written directly: padding rows'
- * scales stay as they were, sf_rows, rows_cap and total_rows are not used. */
+ * scales stay as they were, sf_rows and total_rows are not used. */
 int msc_moe_permute_quantize(const void* tokens_bf16, const int32_t* ids, const float* weights,
                              const int32_t* rank, const int32_t* group_offsets,
                              const float* input_gs, int tokens, int hidden, int topk,
@@ -424,6 +426,12 @@ int msc_moe_permute_quantize(const void* tokens_bf16, const int32_t* ids, const 
 int msc_moe_unpermute(const void* y, const int32_t* ids, const int32_t* rank,
                       const int32_t* group_offsets, void* out, int tokens, int hidden, int topk,
                       int expert_first, int experts_local, void* stream);
+
+/* The same where y has rows_cap rows: pairs whose row the dispatch left out, at or beyond it, are left
+ * out of the sum too. */
+int msc_moe_unpermute_capped(const void* y, const int32_t* ids, const int32_t* rank,
+                             const int32_t* group_offsets, void* out, int tokens, int hidden, int topk,
+                             int expert_first, int experts_local, int rows_cap, void* stream);
 
 /* w1 for the tokens-on-N form of msc_grouped_gemm_nvfp4_swiglu_ragged: gate and up rows
  * interleaved in blocks of 64, so that every 128 consecutive rows hold both halves of 64 output

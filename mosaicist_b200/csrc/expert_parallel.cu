@@ -26,7 +26,6 @@ namespace msc {
 
 constexpr int kMaxPeers = 16;
 constexpr int kMaxSumTopk = 64;   // pairs of one token the final sum stages
-constexpr uint32_t kStatusEpOverflow = 0x00E00000u;   // a destination row beyond rows_cap
 
 // ---- signalling between ranks ----------------------------------------------------------------
 // Each rank owns a small table of flags, 16 per slot, one per peer, that only the peers write
@@ -141,7 +140,7 @@ ep_offsets_kernel(const int* counts_all, int world, int rank, int experts_total,
       if (el == experts_local - 1) *total_rows = min(off + aligned_total[e], rows_cap);
     }
     if (e == (owner + 1) * experts_local - 1 && off + aligned_total[e] > rows_cap)
-      atomicOr(status, kStatusEpOverflow);
+      atomicOr(status, kStatusRowsOverflow);
   }
 }
 
@@ -188,7 +187,7 @@ __global__ void __launch_bounds__(256) ep_dispatch_kernel(const EpDispatchParams
       if (dest < 0 || dest >= p.rows_cap) {   // never store outside the owner's buffers
         valid = false;
         if (kb == 0) {
-          atomicOr(p.status, kStatusEpOverflow);
+          atomicOr(p.status, kStatusRowsOverflow);
           p.pair_row[entry] = -1;   // the combine skips it
         }
       }
@@ -244,7 +243,7 @@ __global__ void __launch_bounds__(256) ep_dispatch_bulk_kernel(const EpDispatchP
           if (p.row_dest[owner]) p.row_dest[owner][dest] = (p.rank << 26) | (int)entry;
           p.pair_row[entry] = dest;
         } else {
-          atomicOr(p.status, kStatusEpOverflow);
+          atomicOr(p.status, kStatusRowsOverflow);
           p.pair_row[entry] = -1;
         }
       } else {

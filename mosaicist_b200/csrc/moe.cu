@@ -220,7 +220,9 @@ struct PermuteParams {
   uint8_t* sf_rows;              // (rows_cap, hidden/16) row-major staging for the scales, or null
   float* row_weight;             // (rows_cap)
   int* row_token;                // (rows_cap)
+  int* status;
   int entries, hidden, topk, expert_first, experts_local;
+  int rows_cap;                  // rows at or beyond it are left out
 };
 
 constexpr int kMaxTopk = 64;   // pairs of one token the dispatch and combine kernels stage
@@ -260,8 +262,13 @@ __global__ void __launch_bounds__(512) moe_permute_quantize_kernel(const Permute
       if (e >= 0 && e < p.experts_local) {
         g = ld_ordered(p.gs + e);
         dest = ld_ordered(p.group_offsets + e) + ld_ordered(p.rank + token * p.topk + k);
-        p.row_weight[dest] = ld_ordered(p.weights + token * p.topk + k);
-        p.row_token[dest] = (int)token;
+        if (dest < 0 || dest >= p.rows_cap) {
+          dest = -1;
+          atomicOr(reinterpret_cast<unsigned*>(p.status), kStatusRowsOverflow);
+        } else {
+          p.row_weight[dest] = ld_ordered(p.weights + token * p.topk + k);
+          p.row_token[dest] = (int)token;
+        }
       }
       s_dest[buf][k] = dest;
       s_gs[buf][k] = g;
@@ -319,7 +326,7 @@ __global__ void __launch_bounds__(256)
 moe_unpermute_kernel(const __nv_bfloat16* y, const int* ids,
                      const int* rank, const int* group_offsets,
                      __nv_bfloat16* __restrict__ out, int tokens, int hidden, int topk,
-                     int expert_first, int experts_local) {
+                     int expert_first, int experts_local, int rows_cap) {
   grid_dependency_wait();
   grid_launch_dependents();
   __shared__ int s_row[kMaxTopk];
@@ -327,7 +334,8 @@ moe_unpermute_kernel(const __nv_bfloat16* y, const int* ids,
   if ((int)threadIdx.x < topk) {
     const long long entry = token * topk + threadIdx.x;
     const int e = ld_ordered(ids + entry) - expert_first;
-    s_row[threadIdx.x] = (e < 0 || e >= experts_local) ? -1 : ld_ordered(group_offsets + e) + ld_ordered(rank + entry);
+    const int row = (e < 0 || e >= experts_local) ? -1 : ld_ordered(group_offsets + e) + ld_ordered(rank + entry);
+    s_row[threadIdx.x] = row < rows_cap ? row : -1;   // (what the dispatch left out is not in y either)
   }
   __syncthreads();
   const int vecs = hidden >> 3;  // 8 bf16 per thread and step
@@ -489,11 +497,14 @@ int msc_moe_permute_quantize(const void* tokens_bf16, const int32_t* ids, const 
   p.sf_rows = staged ? static_cast<uint8_t*>(sf_rows) : nullptr;
   p.entries = tokens * topk; p.hidden = hidden; p.topk = topk;
   p.expert_first = expert_first; p.experts_local = experts_local;
+  p.rows_cap = rows_cap > 0 ? rows_cap : 0x7fffffff;
   if (topk > msc::kMaxTopk) return msc::fail(MSC_ERR_UNSUPPORTED, "topk=%d exceeds %d", topk, msc::kMaxTopk);
   if (reinterpret_cast<uintptr_t>(a_q) % 16)
     return msc::fail(MSC_ERR_BAD_ARG, "a_q must be 16-byte aligned");
   const int smem = 2 * ((hidden / 2 + hidden / 16 + 15) & ~15);
   if (smem > 200 * 1024) return msc::fail(MSC_ERR_UNSUPPORTED, "hidden=%d: two rows do not fit in shared memory", hidden);
+  p.status = msc::status_word();
+  if (!p.status) return msc::fail(MSC_ERR_CUDA, "status word unavailable on this device");
   if (smem > 48 * 1024)
     if (int rc = msc::allow_dynamic_smem(reinterpret_cast<const void*>(msc::moe_permute_quantize_kernel), 200 * 1024))
       return rc;
@@ -515,9 +526,17 @@ int msc_moe_permute_quantize(const void* tokens_bf16, const int32_t* ids, const 
 int msc_moe_unpermute(const void* y, const int32_t* ids, const int32_t* rank,
                       const int32_t* group_offsets, void* out, int tokens, int hidden, int topk,
                       int expert_first, int experts_local, void* stream) {
+  return msc_moe_unpermute_capped(y, ids, rank, group_offsets, out, tokens, hidden, topk, expert_first, experts_local,
+                                  0x7fffffff, stream);
+}
+
+int msc_moe_unpermute_capped(const void* y, const int32_t* ids, const int32_t* rank,
+                             const int32_t* group_offsets, void* out, int tokens, int hidden, int topk,
+                             int expert_first, int experts_local, int rows_cap, void* stream) {
   if (!y || !ids || !rank || !group_offsets || !out) return msc::fail(MSC_ERR_BAD_ARG, "NULL pointer");
   if (tokens <= 0 || topk <= 0 || experts_local <= 0) return msc::fail(MSC_ERR_BAD_ARG, "sizes must be positive");
   if (hidden <= 0 || hidden % 8) return msc::fail(MSC_ERR_BAD_ARG, "hidden=%d must be a multiple of 8", hidden);
+  if (rows_cap <= 0) return msc::fail(MSC_ERR_BAD_ARG, "rows_cap=%d must be positive", rows_cap);
   if (topk > msc::kMaxTopk) return msc::fail(MSC_ERR_UNSUPPORTED, "topk=%d exceeds %d", topk, msc::kMaxTopk);
   const int sms = msc::num_sms();
   if (sms <= 0) return msc::fail(MSC_ERR_CUDA, "could not query the SM count");
@@ -527,7 +546,7 @@ int msc_moe_unpermute(const void* y, const int32_t* ids, const int32_t* rank,
   else lc.numAttrs = 0;   // thousands of CTAs waiting beside the GEMM before it would only be in its way
   MSC_CUDA_OK(cudaLaunchKernelEx(&lc, msc::moe_unpermute_kernel, static_cast<const __nv_bfloat16*>(y), ids, rank,
                                  group_offsets, static_cast<__nv_bfloat16*>(out), tokens, hidden, topk, expert_first,
-                                 experts_local));
+                                 experts_local, rows_cap));
   return MSC_OK;
 }
 

@@ -16,6 +16,7 @@ constexpr long long kDrainBudgetCycles = 100000000LL;  // ~50 ms, exit-path drai
 
 // status word codes (low byte: which wait gave up)
 constexpr int kStatusTimeout = 0x100;
+constexpr uint32_t kStatusRowsOverflow = 0x00E00000u;   // a destination row beyond rows_cap
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

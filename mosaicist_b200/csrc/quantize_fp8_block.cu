@@ -204,6 +204,7 @@ struct Fp8DispatchParams {
   float* sf;                     // (kblocks, pitch)
   float* row_weight;             // (rows_cap)
   int* row_token;                // (rows_cap)
+  int* status;
   int hidden, kblocks, topk, expert_first, experts_local, rows_cap, pitch;
 };
 
@@ -231,6 +232,7 @@ __global__ void __launch_bounds__(512) moe_permute_quantize_fp8_kernel(const Fp8
         dest = ld_ordered(p.group_offsets + e) + ld_ordered(p.rank + pair);
         if (dest < 0 || dest >= p.rows_cap) {
           dest = -1;
+          atomicOr(reinterpret_cast<unsigned*>(p.status), kStatusRowsOverflow);
         } else {
           p.row_weight[dest] = ld_ordered(p.weights + pair);
           p.row_token[dest] = (int)token;
@@ -384,6 +386,8 @@ int msc_moe_permute_quantize_fp8_block(const void* tokens_bf16, const int32_t* i
   const int smem = 2 * ((hidden + 4 * p.kblocks + 15) & ~15);
   if (smem > 200 * 1024) return fail(MSC_ERR_UNSUPPORTED, "hidden=%d: two rows do not fit in shared memory", hidden);
   if (tokens == 0) return MSC_OK;
+  p.status = status_word();
+  if (!p.status) return fail(MSC_ERR_CUDA, "status word unavailable on this device");
   if (smem > 48 * 1024)
     if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(moe_permute_quantize_fp8_kernel), 200 * 1024)) return rc;
   const int sms = num_sms();

@@ -47,7 +47,7 @@ using OptTensor = std::optional<Tensor>;
   X(msc_grouped_gemm_nvfp4_swiglu_ragged) X(msc_grouped_gemm_mxfp8_ragged) X(msc_quantize_rows)  \
   X(msc_amax_global_scale) X(msc_gemm_f16) X(msc_int4_dequant_bf16)                              \
   X(msc_grouped_gemm_bf16_ragged) X(msc_grouped_gemm_bf16_int4_ragged) X(msc_moe_route_topk)     \
-  X(msc_moe_plan) X(msc_moe_permute_quantize) X(msc_moe_unpermute)                               \
+  X(msc_moe_plan) X(msc_moe_permute_quantize) X(msc_moe_unpermute_capped)                        \
   X(msc_moe_masked_workspace) X(msc_moe_masked) X(msc_moe_route) X(msc_moe_route_backward)       \
   X(msc_fp8_block_quantize) X(msc_fp8_block_quantize_weight) X(msc_gemm_fp8_block)               \
   X(msc_grouped_gemm_fp8_block_ragged) X(msc_moe_permute_quantize_fp8_block)
@@ -1086,11 +1086,14 @@ PY_FUNCTION(moe_combine, 3) {
   if (!out) out = empty({T, h}, at::kBFloat16, tokens);
   else need_room(*out, "out", kBf16, T * h);
   const int64_t K = layer.num(s_topk), first = layer.num(s_expert_first), E = layer.num(s_E);
-  const void* y = layer.p<void>(s_y);
+  const Tensor& y = layer.t(s_y);
+  need_room(y, "y", kBf16, h);
+  if (h < 1) value_error("h must be positive");
+  const int cap = as_int(y.numel() / h, "rows of y");    // rows that the dispatch found no room for are not in y
   const int32_t *ids = layer.p<int32_t>(s_ids), *rank = layer.p<int32_t>(s_rank), *offsets = layer.p<int32_t>(s_group_offsets);
   const Lib& f = lib();
   void* st = stream();
-  launch([&] { return f.msc_moe_unpermute(y, ids, rank, offsets, out->data_ptr(), T, h, K, first, E, st); });
+  launch([&] { return f.msc_moe_unpermute_capped(ptr(y), ids, rank, offsets, out->data_ptr(), T, h, K, first, E, cap, st); });
   return wrap(*out);
 }
 

@@ -124,7 +124,8 @@ class MegaMoE:
                  rows_cap: int | None = None, workspace: dict | None = None,
                  gemm1_tokens_on_n: bool | None = None, route: RouteConfig | None = None, route_bias=None):
         """`rows_cap` overrides the row capacity of the grouped buffers (default: room for
-        max_tokens * topk rows plus 127 padding rows per expert); `workspace` may provide the
+        max_tokens * topk rows plus 127 padding rows per expert); a call that needs more leaves the pairs
+        that do not fit out of the sum and raises bit 0x00E00000 in `_lib.status_word()`.  `workspace` may provide the
         buffers other GPUs access under expert parallelism (a_q, a_sf, row_weight, y).  `route` and
         `route_bias` (experts_total,) f32: see RouteConfig; without them the plain rule."""
         self.route_config = RouteConfig() if route is None and route_bias is not None else route
@@ -245,7 +246,9 @@ class MegaMoEFp8Block:
     def __init__(self, w1_q, w1_sf, w2_q, w2_sf, topk: int, max_tokens: int, expert_first: int = 0,
                  route: RouteConfig = RouteConfig(), route_bias=None, rows_cap: int | None = None):
         """`route` and `route_bias` (experts_total,) f32: see RouteConfig.  `rows_cap` overrides the row capacity
-        of the grouped buffers (default: room for max_tokens * topk rows plus 127 padding rows per expert)."""
+        of the grouped buffers (default: room for max_tokens * topk rows plus 127 padding rows per expert); a call
+        that needs more leaves the pairs that do not fit out of the sum and raises bit 0x00E00000 in
+        `_lib.status_word()`."""
         if w1_q.dim() != 3 or w2_q.dim() != 3 or w1_q.shape[1] % 2 or tuple(w2_q.shape) != (
                 w1_q.shape[0], w1_q.shape[2], w1_q.shape[1] // 2):
             raise ValueError(f"w1_q {tuple(w1_q.shape)} and w2_q {tuple(w2_q.shape)} are not (E, 2n, h) and (E, h, n)")

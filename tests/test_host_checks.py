@@ -78,6 +78,18 @@ def test_routed_layer_buffers():
     _refused(lambda b: _host_ops.moe_combine(layer, tokens, b), *_bad(T, h, BF16, F32))
 
 
+def test_routed_layer_result_rows():
+    """The rows that the combine reads are those that y has."""
+    from mosaicist_b200.moe import _host_ops
+
+    T, h, k = 16, 256, 2
+    i32 = lambda *s: _t(*s, dtype=I32)
+    for y in (_t(1152, h, dtype=F32), _t(h, 1152).t(), _t(1152, h, device="cpu"), _t(0, h)):
+        layer = SimpleNamespace(ids=i32(T, k), rank=i32(T, k), group_offsets=i32(8), topk=k, E=8, expert_first=0, h=h, y=y)
+        with pytest.raises(ValueError, match="y "):
+            _host_ops.moe_combine(layer, _t(T, h), _t(T, h))
+
+
 def test_layer_attributes_may_be_computed():
     """A buffer that only the attribute look-up itself holds stays alive for the call."""
     from mosaicist_b200.moe import _host_ops

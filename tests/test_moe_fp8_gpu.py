@@ -208,3 +208,84 @@ def test_one_expert_parallel_rank_equals_the_layer():
         assert torch.equal(ExpertParallelMoE(share, E, k).forward(x, logits), want)
     finally:
         dist.destroy_process_group()
+
+
+def _in_rows_cap(ids, first, local, cap):
+    """The pairs that fit, the others' ids -1 (later rows of an expert are later tokens', so the ranks stay)."""
+    rank, rows, offs, _ = M.plan(ids, first, local)
+    e = ids - first
+    here = (e >= 0) & (e < local)
+    fits = here & (offs[np.where(here, e, 0)] + np.where(here, rank, 0) < cap)
+    assert (here & ~fits).any() and fits.any()
+    return np.where(fits, ids, -1).astype(np.int32)
+
+
+def _guarded(rows, cols, dtype, fill):
+    """A buffer of `rows` rows with 64 rows behind it that nobody may read or write."""
+    whole = torch.empty((rows + 64, cols) if cols else (rows + 64,), dtype=dtype, device="cuda")
+    whole.fill_(fill)
+    return whole, whole[:rows]
+
+
+def test_a_small_rows_cap_leaves_pairs_out():
+    """More rows than rows_cap: nothing is read or written behind the buffers, the pairs that do not fit are missing from
+    the sum and the status word says so."""
+    from mosaicist_b200 import _lib
+    from mosaicist_b200.moe import MegaMoEFp8Block
+
+    E, h, n, k, tokens, cap = 4, 256, 128, 2, 300, 384
+    rng = np.random.default_rng(6)
+    w = _weights(E, h, n, 7)
+    x = rng.standard_normal((tokens, h)).astype(np.float32).astype(ml_dtypes.bfloat16)
+    logits = rng.standard_normal((tokens, E)).astype(np.float32)
+    ids, weights = R.route(logits, k)
+    weights = weights.astype(np.float32).astype(np.float64)
+    layer = MegaMoEFp8Block(*(T(v) for v in w), topk=k, max_tokens=tokens, rows_cap=cap)
+    guards = []
+    for name, cols, dtype, fill in (("a_q", h, torch.uint8, 0x7f), ("row_weight", 0, torch.float32, torch.nan), ("row_token", 0, torch.int32, -9),
+                                    ("gateup", 2 * n, torch.bfloat16, torch.nan), ("d_q", n, torch.uint8, 0x7f), ("y", h, torch.bfloat16, torch.nan)):
+        whole, part = _guarded(cap, cols, dtype, fill)
+        setattr(layer, name, part)
+        guards.append((name, whole[cap:], whole[cap:].clone()))
+    tx, tl = T(x.view(np.int16)).view(torch.bfloat16), T(logits)
+    got = layer.forward(tx, tl)
+    assert _lib.status_word() == 0x00E00000
+    for name, now, before in guards:
+        assert torch.equal(now.view(torch.uint8), before.view(torch.uint8)), name
+    want = _layer(x.astype(np.float32), _in_rows_cap(ids, 0, E, cap), weights, w)
+    scale = np.abs(want).max()
+    assert np.abs(got.double().cpu().numpy() - want).max() < 3e-2 * scale
+    layer = MegaMoEFp8Block(*(T(v) for v in w), topk=k, max_tokens=tokens)
+    _close(layer.forward(tx, tl).double().cpu().numpy(), _layer(x.astype(np.float32), ids, weights, w))
+
+
+def test_a_small_rows_cap_of_the_nvfp4_layer():
+    from mosaicist_b200 import _lib, ops
+    from mosaicist_b200.moe import MegaMoE, RouteConfig
+
+    E, h, n, k, cap = 4, 256, 256, 2, 384
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w1, w2 = (0.05 * torch.randn(s, device="cuda", generator=g) for s in ((E, 2 * n, h), (E, h, n)))
+    ones = torch.ones(E, device="cuda")
+    gs1, gs2 = ops.global_scale_for(w1), ops.global_scale_for(w2)
+    args = (*ops.quantize_nvfp4(w1, gs1), gs1, ones, *ops.quantize_nvfp4(w2, gs2), gs2, ones, 300 * ones, 300 * ones)
+    for tokens in (300, 2500):                                 # scales written in place, and staged by rows
+        x, logits = torch.randn(tokens, h, device="cuda", generator=g).bfloat16(), torch.randn(tokens, E, device="cuda", generator=g)
+        small = MegaMoE(*args, topk=k, max_tokens=tokens, rows_cap=cap, route=RouteConfig())
+        guards = []
+        for name, cols, dtype, fill in (("a_q", h // 2, torch.uint8, 0x77), ("row_weight", 0, torch.float32, torch.nan),
+                                        ("row_token", 0, torch.int32, -9), ("sf_rows", h // 16, torch.uint8, 0x7f), ("y", h, torch.bfloat16, torch.nan)):
+            whole, part = _guarded(cap, cols, dtype, fill)
+            setattr(small, name, part)
+            guards.append((name, whole[cap:], whole[cap:].clone()))
+        got = small.forward(x, logits)
+        assert _lib.status_word() == 0x00E00000
+        for name, now, before in guards:
+            assert torch.equal(now.view(torch.uint8), before.view(torch.uint8)), name
+        full = MegaMoE(*args, topk=k, max_tokens=tokens, route=RouteConfig())
+        full.route(logits)
+        full.ids[:tokens] = T(_in_rows_cap(full.ids[:tokens].cpu().numpy(), 0, E, cap))
+        want = full.forward(x)
+        assert _lib.status_word() == 0
+        assert (got.float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
+        assert (want != 0).any()
