@@ -151,8 +151,6 @@ void launch(F&& f) {
   check(code);
 }
 
-void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
-
 // ---- argument checks ---------------------------------------------------------------------------
 
 enum Types { kBytes, kF32, kI32, kBf16, kBf16F32, kU8, kPackedInt, kFloats, kE4m3 };
@@ -230,8 +228,8 @@ int dt(const Tensor& x) { return x.scalar_type() == at::kBFloat16 ? 0 : 1; }
 int dt3(const Tensor& x) { return x.scalar_type() == at::kHalf ? 2 : dt(x); }
 constexpr at::ScalarType kOutTypes[] = {at::kBFloat16, at::kFloat, at::kHalf};
 
-// Every tensor of a call on the device of the first; the launch then runs there, on that device's
-// current stream, whatever device is current.
+// Every launch runs on the device of the call's (first) tensor, on that device's current stream, whatever device is
+// current: the steps of a layer are then in order.
 void one_device(const Tensor& first, std::initializer_list<std::pair<const Tensor*, const char*>> rest) {
   for (const auto& [t, name] : rest)
     if (C10_UNLIKELY(t && t->device() != first.device()))
@@ -266,10 +264,10 @@ Tensor gemm_masked(const Tensor& a_q, const Tensor& a_sf, const Tensor& b_q, con
   if (out) need(*out, "out", kBf16, {l, m, n});
   else out = empty({l, m, n}, at::kBFloat16, a_q);
   const Lib& f = lib();
-  void* st = stream();
+  const OnDeviceOf on(a_q);
   launch([&] {
     return f.msc_grouped_gemm_nvfp4(ptr(a_q), ptr(a_sf), ptr(b_q), ptr(b_sf), ptr<float>(alpha), ptr<int32_t>(masked_m),
-                                    out->data_ptr(), l, m, n, k, &cfg, st);
+                                    out->data_ptr(), l, m, n, k, &cfg, on.stream);
   });
   return *out;
 }
@@ -295,11 +293,11 @@ Tensor gemm_ragged(bool mxfp8, const Tensor& a_q, const Tensor& a_sf, const Tens
   else out = empty({total, n}, at::kBFloat16, a_q);
   cfg.epilogue = row_scale ? MSC_EPI_ROW_SCALE : MSC_EPI_PLAIN;
   const Lib& f = lib();
-  void* st = stream();
+  const OnDeviceOf on(a_q);
   const auto fn = mxfp8 ? f.msc_grouped_gemm_mxfp8_ragged : f.msc_grouped_gemm_nvfp4_ragged;
   launch([&] {
     return fn(ptr(a_q), ptr(a_sf), ptr(b_q), ptr(b_sf), ptr<float>(alpha), ptr<int32_t>(offsets), ptr<int32_t>(rows),
-              ptr<float>(row_scale), out->data_ptr(), l, total, n, k, &cfg, st);
+              ptr<float>(row_scale), out->data_ptr(), l, total, n, k, &cfg, on.stream);
   });
   return *out;
 }
@@ -327,11 +325,11 @@ std::tuple<Tensor, Tensor> swiglu_ragged(const Tensor& a_q, const Tensor& a_sf, 
     d_sf = at::zeros({(total + 127) / 128, n / 64, 32, 16}, a_q.options().dtype(at::kByte));
   }
   const Lib& f = lib();
-  void* st = stream();
+  const OnDeviceOf on(a_q);
   launch([&] {
     return f.msc_grouped_gemm_nvfp4_swiglu_ragged(ptr(a_q), ptr(a_sf), ptr(w1_q), ptr(w1_sf), ptr<float>(alpha),
                                                   ptr<int32_t>(offsets), ptr<int32_t>(rows), ptr<float>(gs), d_q->data_ptr(),
-                                                  d_sf->data_ptr(), l, total, n2, k, &cfg, st);
+                                                  d_sf->data_ptr(), l, total, n2, k, &cfg, on.stream);
   });
   return {*d_q, *d_sf};
 }
@@ -347,10 +345,10 @@ std::tuple<Tensor, Tensor> quantize_nvfp4(const Tensor& x, const Tensor& gs, con
   Tensor q = empty({l, m, k / 2}, at::kByte, x);
   Tensor sf = tiled ? empty({l, m / 128, k / 64, 32, 16}, at::kByte, x) : empty({l, m, k / 16}, at::kByte, x);
   const Lib& f = lib();
-  void* st = stream();
+  const OnDeviceOf on(x);
   launch([&] {
     return f.msc_quantize_rows(0, ptr(x), silu ? 2 : dt(x), ptr<float>(gs), nullptr, ptr<int32_t>(masked_m), q.data_ptr(),
-                               sf.data_ptr(), (tiled ? 1 : 0) | MSC_SF_ZERO_REST, nullptr, l, l * m, m, k, st);
+                               sf.data_ptr(), (tiled ? 1 : 0) | MSC_SF_ZERO_REST, nullptr, l, l * m, m, k, on.stream);
   });
   return {q, sf};
 }
@@ -373,10 +371,10 @@ std::tuple<Tensor, Tensor> quantize_nvfp4_ragged(const Tensor& x, const Tensor& 
     need(*sf, "sf", kU8, {(total + 127) / 128, k / 64, 32, 16});
   }
   const Lib& f = lib();
-  void* st = stream();
+  const OnDeviceOf on(x);
   launch([&] {
     return f.msc_quantize_rows(0, ptr(x), silu ? 2 : dt(x), ptr<float>(gs), ptr<int32_t>(offsets), ptr<int32_t>(rows),
-                               q->data_ptr(), sf->data_ptr(), 1 | (fresh ? MSC_SF_ZERO_REST : 0), nullptr, l, total, 0, k, st);
+                               q->data_ptr(), sf->data_ptr(), 1 | (fresh ? MSC_SF_ZERO_REST : 0), nullptr, l, total, 0, k, on.stream);
   });
   return {*q, *sf};
 }
@@ -388,9 +386,9 @@ Tensor global_scale_for(const Tensor& x, double numerator, OptTensor out) {
   if (out) need(*out, "out", kF32, {l});
   else out = empty({l}, at::kFloat, x);
   const Lib& f = lib();
-  void* st = stream();
+  const OnDeviceOf on(x);
   launch([&] {
-    return f.msc_amax_global_scale(ptr(x), dt(x), l, x.numel() / l, (float)numerator, static_cast<float*>(out->data_ptr()), st);
+    return f.msc_amax_global_scale(ptr(x), dt(x), l, x.numel() / l, (float)numerator, static_cast<float*>(out->data_ptr()), on.stream);
   });
   return *out;
 }
@@ -417,11 +415,11 @@ std::tuple<Tensor, Tensor> quantize_mxfp8(const Tensor& x, bool tiled, const Opt
     need_room(*sf, "sf", kBytes, tiled ? (total + 127) / 128 * (k / 128) * 512 : total * (k / 32));
   }
   const Lib& f = lib();
-  void* st = stream();
+  const OnDeviceOf on(x);
   launch([&] {
     return f.msc_quantize_rows(1, ptr(x), dt(x), nullptr, ptr<int32_t>(offsets), offsets ? ptr<int32_t>(rows) : nullptr,
                                q->data_ptr(), sf->data_ptr(), (tiled ? 1 : 0) | (fresh ? MSC_SF_ZERO_REST : 0), nullptr, l,
-                               total, 0, k, st);
+                               total, 0, k, on.stream);
   });
   return {*q, *sf};
 }
@@ -439,10 +437,10 @@ Tensor gemm_f16(const Tensor& a, const Tensor& b, OptTensor out, int max_ctas) {
   else if (!out->is_cuda() || out->scalar_type() != t || out->dim() != 2 || out->size(0) != m || out->size(1) != n || out->stride(1) != 1)
     value_error("out must be an (m, n) CUDA tensor in the input dtype with unit stride along rows");
   const Lib& f = lib();
-  void* st = stream();
+  const OnDeviceOf on(a);
   launch([&] {
     return f.msc_gemm_f16(ptr(a), ptr(b), out->data_ptr(), m, n, k, a.stride(0), b.stride(0), out->stride(0),
-                          t == at::kHalf ? 0 : 1, max_ctas, st);
+                          t == at::kHalf ? 0 : 1, max_ctas, on.stream);
   });
   return *out;
 }
@@ -456,8 +454,8 @@ Tensor dequant_int4(const Tensor& b_q, const Tensor& scales, int64_t group_size,
   if (!out) out = empty({l, n, k}, at::kBFloat16, b_q);
   else need_room(*out, "out", kBf16, l * n * k);
   const Lib& f = lib();
-  void* st = stream();
-  launch([&] { return f.msc_int4_dequant_bf16(ptr(b_q), ptr(scales), out->data_ptr(), l, n, k, group_size, st); });
+  const OnDeviceOf on(b_q);
+  launch([&] { return f.msc_int4_dequant_bf16(ptr(b_q), ptr(scales), out->data_ptr(), l, n, k, group_size, on.stream); });
   return *out;
 }
 
@@ -474,10 +472,10 @@ Tensor gemm_bf16_ragged(const Tensor& a, const Tensor& b, const Tensor& offsets,
   if (!out) out = empty({total, n}, at::kBFloat16, a);
   else need_room(*out, "out", kBf16, total * n);
   const Lib& f = lib();
-  void* st = stream();
+  const OnDeviceOf on(a);
   launch([&] {
     return f.msc_grouped_gemm_bf16_ragged(ptr(a), ptr(b), ptr<float>(alpha), ptr<int32_t>(offsets), ptr<int32_t>(rows),
-                                          out->data_ptr(), l, total, n, k, max_ctas, st);
+                                          out->data_ptr(), l, total, n, k, max_ctas, on.stream);
   });
   return *out;
 }
@@ -508,10 +506,10 @@ Tensor gemm_int4_ragged(const Tensor& a, const Tensor& b_q, const Tensor& scales
   if (!out) out = empty({total, n}, at::kBFloat16, a);
   else need_room(*out, "out", kBf16, total * n);
   const Lib& f = lib();
-  void* st = stream();
+  const OnDeviceOf on(a);
   launch([&] {
     return f.msc_grouped_gemm_bf16_int4_ragged(ptr(a), ptr(b_q), ptr(scales), ptr<float>(alpha), ptr<int32_t>(offsets),
-                                               ptr<int32_t>(rows), out->data_ptr(), l, total, n, k, group_size, max_ctas, st);
+                                               ptr<int32_t>(rows), out->data_ptr(), l, total, n, k, group_size, max_ctas, on.stream);
   });
   return *out;
 }
@@ -719,15 +717,15 @@ OptTensor moe_masked(const Tensor& hidden, const Tensor& w1_q, const Tensor& w1_
   need(w2_sf, "b_sf", kBytes, {l, k / 128, n / 64, 32, 16});
   need(a2_gs, "out_global_scale", kF32, {l});
   const Lib& f = lib();
+  const OnDeviceOf on(hidden);
   const size_t bytes = f.msc_moe_masked_workspace(l, m, k, n);
   Tensor ws = empty({(int64_t)bytes}, at::kByte, hidden);
   Tensor out = empty({l, m, k}, at::kBFloat16, hidden);
-  void* st = stream();
   launch([&] {
     return f.msc_moe_masked(ptr(hidden), ptr(w1_q), ptr(w1_sf), ptr<float>(w1_gs), ptr<float>(w1_alpha), ptr(w2_q), ptr(w2_sf),
                             ptr<float>(w2_gs), ptr<float>(w2_alpha), ptr<int32_t>(masked_m), ptr<float>(in_gs),
                             ptr<float>(a2_gs), ptr<float>(g1_alpha), ptr<float>(g2_alpha), ws.data_ptr(), bytes,
-                            out.data_ptr(), zero_rest ? 1 : 0, l, m, k, n, st);
+                            out.data_ptr(), zero_rest ? 1 : 0, l, m, k, n, on.stream);
   });
   return out;
 }
@@ -987,13 +985,16 @@ void route(Layer& layer, const Tensor& logits) {
   need_dim(logits, "logits", 2);
   const int64_t tokens = logits.size(0), experts = logits.size(1), topk = layer.num(s_topk);
   need_room(logits, "logits", kF32, tokens * experts);
-  need_room(layer.t(s_ids), "ids", kI32, tokens * topk);
-  need_room(layer.t(s_weights), "weights", kF32, tokens * topk);
-  int32_t* ids = layer.p<int32_t>(s_ids);
-  float* weights = layer.p<float>(s_weights);
+  const Tensor &ids = layer.t(s_ids), &weights = layer.t(s_weights);
+  need_room(ids, "ids", kI32, tokens * topk);
+  need_room(weights, "weights", kF32, tokens * topk);
+  one_device(logits, {{&ids, "ids"}, {&weights, "weights"}});
   const Lib& f = lib();
-  void* st = stream();
-  launch([&] { return f.msc_moe_route_topk(ptr<float>(logits), ids, weights, tokens, experts, topk, st); });
+  const OnDeviceOf on(logits);
+  launch([&] {
+    return f.msc_moe_route_topk(ptr<float>(logits), static_cast<int32_t*>(ids.data_ptr()), static_cast<float*>(weights.data_ptr()),
+                                tokens, experts, topk, on.stream);
+  });
 }
 
 // route(self, logits)
@@ -1017,20 +1018,23 @@ PY_FUNCTION(moe_dispatch, 3) {
   if (tokens.numel() != T * h) value_error("tokens has shape " + shape_text(tokens.sizes()) + ", expected " + shape_text({T, h}));
   for (PyObject* name : {s_ids, s_rank}) need_room(layer.t(name), "ids / rank", kI32, T * K);
   if (a[2] != Py_None) route(layer, tensor(a[2], "logits"));
-  int32_t *ids = layer.p<int32_t>(s_ids), *rank = layer.p<int32_t>(s_rank), *rows = layer.p<int32_t>(s_group_rows);
-  int32_t *offsets = layer.p<int32_t>(s_group_offsets), *total = layer.p<int32_t>(s_total_rows), *scratch = layer.p<int32_t>(s_scratch);
-  const Tensor* staged = layer.opt(s_sf_rows);
-  void* sf_rows = staged ? staged->data_ptr() : nullptr;
-  const float *weights = layer.p<float>(s_weights), *gs = layer.p<float>(s_input_gs);
-  void *a_q = layer.p<void>(s_a_q), *a_sf = layer.p<void>(s_a_sf);
-  float* row_weight = layer.p<float>(s_row_weight);
-  int32_t* row_token = layer.p<int32_t>(s_row_token);
+  const Tensor &ids = layer.t(s_ids), &weights = layer.t(s_weights), &rank = layer.t(s_rank), &rows = layer.t(s_group_rows);
+  const Tensor &offsets = layer.t(s_group_offsets), &total = layer.t(s_total_rows), &scratch = layer.t(s_scratch);
+  const Tensor &gs = layer.t(s_input_gs), &a_q = layer.t(s_a_q), &a_sf = layer.t(s_a_sf), &row_weight = layer.t(s_row_weight);
+  const Tensor &row_token = layer.t(s_row_token), *sf_rows = layer.opt(s_sf_rows);
+  one_device(tokens, {{&ids, "ids"}, {&weights, "weights"}, {&rank, "rank"}, {&rows, "group_rows"}, {&offsets, "group_offsets"},
+                      {&total, "total_rows"}, {&scratch, "scratch"}, {&gs, "input_gs"}, {&a_q, "a_q"}, {&a_sf, "a_sf"},
+                      {&row_weight, "row_weight"}, {&row_token, "row_token"}, {sf_rows, "sf_rows"}});
   const Lib& f = lib();
-  void* st = stream();
-  launch([&] { return f.msc_moe_plan(ids, T * K, first, E, rank, rows, offsets, total, scratch, st); });
+  const OnDeviceOf on(tokens);
+  auto i32 = [](const Tensor& v) { return static_cast<int32_t*>(v.data_ptr()); };
   launch([&] {
-    return f.msc_moe_permute_quantize(ptr(tokens), ids, weights, rank, offsets, gs, T, h, K, first, E, a_q, a_sf, row_weight,
-                                      row_token, sf_rows, cap, total, st);
+    return f.msc_moe_plan(i32(ids), T * K, first, E, i32(rank), i32(rows), i32(offsets), i32(total), i32(scratch), on.stream);
+  });
+  launch([&] {
+    return f.msc_moe_permute_quantize(ptr(tokens), i32(ids), ptr<float>(weights), i32(rank), i32(offsets), ptr<float>(gs), T, h, K,
+                                      first, E, a_q.data_ptr(), a_sf.data_ptr(), static_cast<float*>(row_weight.data_ptr()),
+                                      i32(row_token), sf_rows ? sf_rows->data_ptr() : nullptr, cap, i32(total), on.stream);
   });
   Py_RETURN_NONE;
 }
@@ -1090,10 +1094,17 @@ PY_FUNCTION(moe_combine, 3) {
   need_room(y, "y", kBf16, h);
   if (h < 1) value_error("h must be positive");
   const int cap = as_int(y.numel() / h, "rows of y");    // rows that the dispatch found no room for are not in y
-  const int32_t *ids = layer.p<int32_t>(s_ids), *rank = layer.p<int32_t>(s_rank), *offsets = layer.p<int32_t>(s_group_offsets);
+  const Tensor &ids = layer.t(s_ids), &rank = layer.t(s_rank), &offsets = layer.t(s_group_offsets);
+  need_room(ids, "ids", kI32, T * K);
+  need_room(rank, "rank", kI32, T * K);
+  need_room(offsets, "group_offsets", kI32, E);
+  one_device(y, {{&tokens, "tokens"}, {&ids, "ids"}, {&rank, "rank"}, {&offsets, "group_offsets"}, {&*out, "out"}});
   const Lib& f = lib();
-  void* st = stream();
-  launch([&] { return f.msc_moe_unpermute_capped(ptr(y), ids, rank, offsets, out->data_ptr(), T, h, K, first, E, cap, st); });
+  const OnDeviceOf on(y);
+  launch([&] {
+    return f.msc_moe_unpermute_capped(ptr(y), ptr<int32_t>(ids), ptr<int32_t>(rank), ptr<int32_t>(offsets), out->data_ptr(), T, h, K,
+                                      first, E, cap, on.stream);
+  });
   return wrap(*out);
 }
 

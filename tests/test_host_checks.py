@@ -90,6 +90,46 @@ def test_routed_layer_result_rows():
             _host_ops.moe_combine(layer, _t(T, h), _t(T, h))
 
 
+def test_routed_layer_buffers_of_another_device():
+    from mosaicist_b200.moe import _host_ops
+
+    T, h, E, k = 16, 256, 8, 2
+    i32 = lambda *s: _t(*s, dtype=I32)
+    buffers = dict(ids=i32(T, k), weights=_t(T, k, dtype=F32), rank=i32(T, k), group_rows=i32(E), group_offsets=i32(E), total_rows=i32(1),
+                   scratch=i32(4), input_gs=_t(E, dtype=F32), a_q=_t(1152, h // 2, dtype=U8), a_sf=_t(9, h // 64, 32, 16, dtype=U8),
+                   row_weight=_t(1152, dtype=F32), row_token=i32(1152), sf_rows=_t(1152, h // 16, dtype=U8), y=_t(1152, h))
+    sizes = dict(topk=k, E=E, expert_first=0, h=h, rows_cap=1152)
+    tokens, logits, other = _t(T, h), _t(T, E, dtype=F32), torch.device("cuda", 1)
+    for name, b in buffers.items():
+        layer = SimpleNamespace(**buffers | sizes | {name: torch.empty(b.shape, dtype=b.dtype, device=other)})
+        if name != "y":
+            with pytest.raises(ValueError, match=f"{name} is on cuda:1, expected cuda:0"):
+                _host_ops.moe_dispatch(layer, tokens, None)
+        if name in ("ids", "weights"):
+            with pytest.raises(ValueError, match=f"{name} is on cuda:1, expected cuda:0"):
+                _host_ops.moe_route(layer, logits)
+        if name in ("ids", "rank", "group_offsets", "y"):
+            with pytest.raises(ValueError, match="is on cuda:[01], expected cuda:[01]"):
+                _host_ops.moe_combine(layer, tokens, _t(T, h))
+    layer = SimpleNamespace(**buffers | sizes)
+    with pytest.raises(ValueError, match="out is on cuda:1"):
+        _host_ops.moe_combine(layer, tokens, _t(T, h, device=other))
+    with pytest.raises(ValueError, match="tokens is on cuda:1"):
+        _host_ops.moe_combine(layer, _t(T, h, device=other), _t(T, h))
+
+
+def test_every_launch_names_the_device_it_runs_on():
+    """Nothing takes the stream of whatever device is current: a property of the source, so it is checked there."""
+    import pathlib
+    import re
+
+    text = (pathlib.Path(__file__).resolve().parents[1] / "mosaicist_b200" / "host_ops" / "host_ops.cpp").read_text()
+    assert not re.search(r"getCurrentCUDAStream\(\s*\)", text)
+    for body in re.split(r"^\}[^\n]*$", re.sub(r"//[^\n]*", "", text), flags=re.M):
+        if "launch([&]" in body:
+            assert "const OnDeviceOf on(" in body and "on.stream" in body, body
+
+
 def test_layer_attributes_may_be_computed():
     """A buffer that only the attribute look-up itself holds stays alive for the call."""
     from mosaicist_b200.moe import _host_ops
