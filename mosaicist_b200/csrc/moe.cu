@@ -505,7 +505,7 @@ int msc_moe_permute_quantize(const void* tokens_bf16, const int32_t* ids, const 
   if (smem > 200 * 1024) return msc::fail(MSC_ERR_UNSUPPORTED, "hidden=%d: two rows do not fit in shared memory", hidden);
   p.status = msc::status_word();
   if (!p.status) return msc::fail(MSC_ERR_CUDA, "status word unavailable on this device");
-  if (smem > 48 * 1024)
+  if (smem + (int)sizeof(int) * 4 * msc::kMaxTopk > 48 * 1024)   // (with its static arrays)
     if (int rc = msc::allow_dynamic_smem(reinterpret_cast<const void*>(msc::moe_permute_quantize_kernel), 200 * 1024))
       return rc;
   // enough CTAs to fill every SM (16 x 128 threads), each walking its share of the tokens; wide CTAs

@@ -388,7 +388,7 @@ int msc_moe_permute_quantize_fp8_block(const void* tokens_bf16, const int32_t* i
   if (tokens == 0) return MSC_OK;
   p.status = status_word();
   if (!p.status) return fail(MSC_ERR_CUDA, "status word unavailable on this device");
-  if (smem > 48 * 1024)
+  if (smem + (int)sizeof(int) * 2 * kFp8MaxTopk > 48 * 1024)   // (with its static arrays)
     if (int rc = allow_dynamic_smem(reinterpret_cast<const void*>(moe_permute_quantize_fp8_kernel), 200 * 1024)) return rc;
   const int sms = num_sms();
   if (sms <= 0) return fail(MSC_ERR_CUDA, "could not query the SM count");

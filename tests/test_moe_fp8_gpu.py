@@ -289,3 +289,9 @@ def test_a_small_rows_cap_of_the_nvfp4_layer():
         assert _lib.status_word() == 0
         assert (got.float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
         assert (want != 0).any()
+
+
+@pytest.mark.parametrize("h", [23584, 23808, 24576])
+def test_dispatch_of_rows_that_nearly_fill_the_default_shared_memory(h):
+    """Two rows of 23584 to 23824 columns are under 48 KB, with the kernel's own arrays they are not."""
+    test_dispatch_bit_exact(3, h, 8, 2, 0, 8)

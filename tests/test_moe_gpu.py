@@ -423,3 +423,9 @@ def test_dispatch_and_combine_forms_agree(tokens_n):
     assert torch.equal(_host_ops.moe_combine(layer, x[:few], None), out[:few])
     assert int((out != 0).sum()) > out.numel() // 2
     assert _lib.status_word() == 0
+
+
+@pytest.mark.parametrize("h", [42816, 43648])
+def test_gather_quantise_of_rows_that_nearly_fill_the_default_shared_memory(h):
+    """Two rows of 42816 to 43648 columns are under 48 KB, with the kernel's own arrays they are not."""
+    test_plan_and_gather_quantise_bit_exact(0, 4, h, False)
