@@ -317,7 +317,8 @@ int msc_fp8_block_quantize_weight(const void* w, int w_dtype, void* q, float* sf
 
 /* out (m, n) = dequant(a) (m, k) x dequant(b) (n, k)^T, fp32 sums, out_dtype as above.  a_sf as
  * msc_fp8_block_quantize lays it out (pitch = m rounded up to 4), b_sf (ceil(n / 128), ceil(k / 128)).
- * n % 8 == 0.  max_ctas: CTAs of the launch, 0 = all SMs.  m = 0 does nothing. */
+ * n % 8 == 0; a_q, a_sf, b_q and out are 16-byte aligned.  max_ctas: CTAs of the launch, 0 = all SMs.  m = 0
+ * does nothing. */
 int msc_gemm_fp8_block(const void* a_q, const float* a_sf, const void* b_q, const float* b_sf, void* out,
                        int out_dtype, int m, int n, int k, int max_ctas, void* stream);
 

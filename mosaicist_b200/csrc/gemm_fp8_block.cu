@@ -82,8 +82,6 @@ struct Fp8Smem {
   static constexpr int kTmemSlot = 1000, kAbort = 1004;
 };
 
-// Rows of a group as the tiles see them: they start at a multiple of 4 (the scales arrive as 16-byte
-// pieces), up to three rows before the group, which are computed and not stored.
 __device__ __forceinline__ void fp8_group(const Fp8Params& p, int g, int& rows, int& off) {
   if (!p.group_rows) {
     rows = p.rows_total;
@@ -91,14 +89,13 @@ __device__ __forceinline__ void fp8_group(const Fp8Params& p, int g, int& rows, 
     return;
   }
   load_group(p.group_rows, p.group_offsets, p.rows_total, g, rows, off);
-  if (rows > 0) rows += off & 3;
 }
 
 __device__ __forceinline__ int fp8_token_tiles(int rows) { return (rows + 255) >> 8; }
 
 struct Fp8Tile {
   int g, nt;        // group, weight tile of 256 rows
-  int row0, lead;   // first token row (a multiple of 4); rows of it that belong to somebody else
+  int row0;         // first token row
   int tn;           // tokens
   bool few;         // the weights are the M side
   int width;        // the N side: weight rows, or tokens where they are few, rounded up to 32
@@ -112,7 +109,6 @@ struct Fp8Cursor {
       const int tt = tid / ntiles;
       tile.g = 0;
       tile.nt = tid - tt * ntiles;
-      tile.lead = 0;
       tile.row0 = tt * 256 + (q & 3) * 64;
       tile.tn = min(p.rows_total - tile.row0, t < p.quarters_from ? 256 : 64);
       shape(p, tile);
@@ -124,8 +120,7 @@ struct Fp8Cursor {
       return false;
     const int u = t - first, tt = u / ntiles;
     tile.nt = u - tt * ntiles;
-    tile.lead = tt == 0 ? (off & 3) : 0;
-    tile.row0 = (off & ~3) + tt * 256;
+    tile.row0 = off + tt * 256;
     tile.tn = min(rows - tt * 256, 256);
     shape(p, tile);
     return true;
@@ -181,9 +176,8 @@ __device__ __forceinline__ void store_value(const Fp8Params& p, size_t at, float
   else if (p.out_type == 1) static_cast<float*>(p.out)[at] = v;
   else static_cast<__half*>(p.out)[at] = __float2half_rn(v);
 }
-// Writes a box of 32 rows x 64 bytes out: rows [first, last) of the matrix, columns col .. of `bytes` each.
-__device__ __forceinline__ void store_box(const Fp8Params& p, uint32_t box, int row0, int first, int last, int col, int bytes,
-                                          int lane) {
+// Writes a box of 32 rows x 64 bytes out: rows [row0, last) of the matrix, columns col .. of `bytes` each.
+__device__ __forceinline__ void store_box(const Fp8Params& p, uint32_t box, int row0, int last, int col, int bytes, int lane) {
   const int piece = lane & 3;
   const bool in = col + piece * (16 / bytes) < p.n;
 #pragma unroll
@@ -193,7 +187,7 @@ __device__ __forceinline__ void store_box(const Fp8Params& p, uint32_t box, int 
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "r"(box + (r * 8 + (lane >> 2)) * Fp8Smem::kBoxPitch + piece * 16) : "memory");
-    if (in && row >= first && row < last)
+    if (in && row < last)
       *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + ((size_t)row * p.n + col) * bytes + piece * 16) = v;
   }
 }
@@ -213,13 +207,13 @@ __device__ __forceinline__ void store_piece(const Fp8Params& p, const Fp8Tile& t
                                             int lane, uint32_t box) {
   const int mine = tile.row0 + (tile.few ? pc * 32 : rank * 128 + quad * 32);
   const float rs = p.row_scale && mine + lane < p.rows_total ? ld_ordered(p.row_scale + mine + lane) : 1.0f;
-  const int first = tile.row0 + tile.lead, last = tile.row0 + tile.tn;
+  const int last = tile.row0 + tile.tn;
   if (tile.few) {   // lanes are neighbouring columns of a token already
     const int col = tile.nt * 256 + rank * 128 + quad * 32 + lane;
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
       const float x = v[e] * __shfl_sync(0xffffffffu, rs, e);
-      if (mine + e >= first && mine + e < last && col < p.n) store_value(p, (size_t)(mine + e) * p.n + col, x);
+      if (mine + e < last && col < p.n) store_value(p, (size_t)(mine + e) * p.n + col, x);
     }
     return;
   }
@@ -237,7 +231,7 @@ __device__ __forceinline__ void store_piece(const Fp8Params& p, const Fp8Tile& t
                      __float_as_uint(x[2] * rs), __float_as_uint(x[3] * rs));
       }
       __syncwarp();
-      store_box(p, box, mine, first, last, col + h * 16, 4, lane);
+      store_box(p, box, mine, last, col + h * 16, 4, lane);
     }
   } else {
     __syncwarp();
@@ -249,7 +243,7 @@ __device__ __forceinline__ void store_piece(const Fp8Params& p, const Fp8Tile& t
       st_shared_v4(box + lane * Fp8Smem::kBoxPitch + i * 16, w[0], w[1], w[2], w[3]);
     }
     __syncwarp();
-    store_box(p, box, mine, first, last, col, 2, lane);
+    store_box(p, box, mine, last, col, 2, lane);
   }
 }
 

@@ -399,3 +399,25 @@ def test_torch_operators():
     offs, rows = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, 20], [10, 15]))
     y = O.grouped_gemm_fp8_block_ragged(q, sf, wq, wsf, offs, rows, None, torch.float16)
     assert torch.equal(y[20:35], want[20:35].half()) and (y[10:20] == 0).all() and (y[35:] == 0).all()
+
+
+@pytest.mark.parametrize("rows", [[64, 64, 64], [256, 256], [63, 65, 62, 64], [255, 257, 256, 1], [512, 64]])
+def test_whole_tiles_at_odd_rows(rows):
+    """Groups of whole tiles that start on any row, a row between them that nobody owns."""
+    from mosaicist_b200 import ops
+
+    n, k = 392, 528
+    offs, at = [], 3
+    for r in rows:
+        offs.append(at)
+        at += r + 1
+    rng = np.random.default_rng(rows)
+    a, sa, b, sb = _operands(rng, at, len(rows), n, k, True)
+    want = np.full((at, n), -3.0)
+    for g, (o, r) in enumerate(zip(offs, rows)):
+        want[o:o + r] = F.product(a[o:o + r], sa[:, o:o + r], b[g], sb[g])[0]
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    for dtype in DT:
+        out = torch.full((at, n), -3.0, dtype=DT[dtype], device="cuda")
+        ops.ragged_grouped_gemm_fp8_block(T(a), _dev_sf(sa), T(b), T(sb), i32(offs), i32(rows), out=out)
+        _check(out, want, None, k, dtype, True)
