@@ -313,8 +313,10 @@ __device__ __forceinline__ float softmax_weight(float x, float ref) {
   return x == ref ? (x == -INFINITY ? 0.0f : 1.0f) : expf(x - ref);
 }
 
-// Sigmoids of so small a logit, e^x each, vanish in fp32 but not in 64 bits: their ratios are e^(x - best).
-__device__ __forceinline__ bool vanishing(float best) { return best < -64.0f && best >= -709.7827f; }
+// Sigmoids of small logits, e^x each to a relative e^-16 (two roundings), lose bits in fp32 below e^-87 and vanish below
+// e^-104, where their share of the sum need not: their ratios are e^(x - best).  Above, what fp32 loses is less than
+// 2^-126 of the sum.  In 64 bits they vanish too below -709.
+__device__ __forceinline__ bool vanishing(float best) { return best < -16.0f && best >= -709.7827f; }
 
 // A bit per slot in which this lane has an expert.
 template <int PER>

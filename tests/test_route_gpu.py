@@ -464,3 +464,16 @@ def test_many_tokens_with_close_keys_beside_barred_biases(E, groups, masks):
         got = ids.cpu().numpy()
         assert not np.isin(got, at[:2]).any()
         assert all(len(set(r)) == len(r) for r in got.tolist())
+
+
+@pytest.mark.parametrize("T", [20, 1040])
+def test_sigmoids_of_which_some_vanish_in_32_bits(T):
+    """The best choice is an ordinary number, others are sub-normal or 0 in fp32; their share of the sum is not."""
+    rng = np.random.default_rng(11)
+    x = np.full((T, 64), -400.0)
+    best = np.array([-10, -16, -17, -20, -40, -60, -63, -64])[np.arange(T) % 8]
+    x[:, 3] = best
+    for e, lo, hi in ((7, -96, -87), (20, -103, -96), (21, -110, -103), (40, -130, -110), (61, -90, -70)):
+        x[:, e] = rng.integers(lo, hi, T)
+    _check(x, 6, score="sigmoid")
+    _check(x, 6, score="sigmoid", scale=2.5, bias=np.zeros(64))
