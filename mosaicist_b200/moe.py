@@ -244,8 +244,8 @@ class MegaMoEFp8Block:
     LOCAL experts; h and n are multiples of 16.  Workspaces are sized for `max_tokens` once."""
 
     def __init__(self, w1_q, w1_sf, w2_q, w2_sf, topk: int, max_tokens: int, expert_first: int = 0,
-                 route: RouteConfig = RouteConfig(), route_bias=None, rows_cap: int | None = None):
-        """`route` and `route_bias` (experts_total,) f32: see RouteConfig.  `rows_cap` overrides the row capacity
+                 route: RouteConfig | None = None, route_bias=None, rows_cap: int | None = None):
+        """`route` and `route_bias` (experts_total,) f32: see RouteConfig; without them the plain rule.  `rows_cap` overrides the row capacity
         of the grouped buffers (default: room for max_tokens * topk rows plus 127 padding rows per expert); a call
         that needs more leaves the pairs that do not fit out of the sum and raises bit 0x00E00000 in
         `_lib.status_word()`."""
@@ -259,7 +259,8 @@ class MegaMoEFp8Block:
         if max_tokens < 1 or not 1 <= topk <= 32:
             raise ValueError("max_tokens must be positive and topk in [1, 32]")
         self.w1_q, self.w1_sf, self.w2_q, self.w2_sf = w1_q, w1_sf, w2_q, w2_sf
-        self.route_config, self.route_bias = route, route_bias
+        self.route_config = RouteConfig() if route is None else route
+        self.route_bias = route_bias
         self.max_tokens = max_tokens
         cap = rows_cap if rows_cap is not None else (max_tokens * topk + 127 * self.E + 127) // 128 * 128
         if cap <= 0 or cap % 128:

@@ -245,3 +245,15 @@ def test_fp8_layer_arguments(fake):
     for call in (lambda: layer.forward(_t(9, 256, dtype=BF16)), lambda: layer.route(_t(9, 4)), lambda: layer.forward(_t(8, 256, dtype=BF16), _t(7, 4))):
         with pytest.raises(ValueError):
             call()
+
+
+def test_fp8_layer_without_a_router_of_its_own(fake, monkeypatch):
+    """route=None is the plain rule, as MegaMoE has it."""
+    from mosaicist_b200 import moe
+
+    w1, s1, w2, s2 = _t(4, 512, 256, dtype=U8), _t(4, 4, 2), _t(4, 256, 256, dtype=U8), _t(4, 2, 2)
+    seen = []
+    monkeypatch.setattr(ops, "moe_route", lambda *args: seen.append(args[1:9]))
+    for kw in (dict(), dict(route=None), dict(route=moe.RouteConfig())):
+        moe.MegaMoEFp8Block(w1, s1, w2, s2, topk=2, max_tokens=8, **kw).route(_t(8, 4))
+    assert seen == [(2, "softmax", None, 1, 1, 1, True, 1.0)] * 3
