@@ -364,7 +364,8 @@ typedef struct msc_route_cfg {
  * its expert; where fewer than topk are left the lowest barred ones fill up, with weight 0.
  * logits (tokens, experts), dtype 0 bf16, 1 f32, 2 f16 -> ids (tokens, topk) i32, weights (tokens, topk) f32.
  * experts <= 1024, groups * ceil(experts / groups / 32) <= 32, topk <= 32 and at most the experts of
- * topk_groups groups.  tokens = 0 does nothing. */
+ * topk_groups groups.  tokens = 0 does nothing but check its arguments (pointers to what is then empty may be
+ * NULL, here and below and in the FP8 block quantiser and products). */
 int msc_moe_route(const void* logits, int dtype, const float* bias, int32_t* ids, float* weights, int tokens,
                   int experts, int topk, const msc_route_cfg* cfg, void* stream);
 

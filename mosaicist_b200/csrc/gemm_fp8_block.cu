@@ -567,7 +567,7 @@ gemm_fp8_block_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_c
 static int gemm_fp8_block(const void* a_q, const float* a_sf, const void* b_q, const float* b_sf,
                           const int32_t* group_offsets, const int32_t* group_rows, const float* row_scale, void* out,
                           int out_type, int l, int rows_total, int n, int k, int max_ctas, void* stream) {
-  if (!a_q || !a_sf || !b_q || !b_sf || !out) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
+  if (!b_q || !b_sf || (rows_total != 0 && (!a_q || !a_sf || !out))) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
   if (l <= 0 || n <= 0 || k <= 0 || rows_total < 0)
     return fail(MSC_ERR_BAD_ARG, "l=%d, n=%d, k=%d must be positive, rows=%d must not be negative", l, n, k, rows_total);
   if (k % 16) return fail(MSC_ERR_BAD_ARG, "k=%d must be a multiple of 16", k);

@@ -882,7 +882,7 @@ extern "C" {
 int msc_moe_route(const void* logits, int dtype, const float* bias, int32_t* ids, float* weights, int tokens,
                   int experts, int topk, const msc_route_cfg* cfg, void* stream) {
   using namespace msc;
-  if (!logits || !ids || !weights || !cfg) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
+  if (!cfg || (tokens != 0 && (!logits || !ids || !weights))) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
   if (int rc = check_route(logits, dtype, tokens, experts, topk, cfg->score, cfg->scale)) return rc;
   if (misaligned(bias, 4) || misaligned(ids, 4) || misaligned(weights, 4))
     return fail(MSC_ERR_BAD_ARG, "bias, ids and weights must be 4-byte aligned");
@@ -921,7 +921,7 @@ int msc_moe_route_backward(const float* grad_weights, const void* logits, int dt
                            const float* weights, void* grad_logits, int tokens, int experts, int topk, int score,
                            int renormalize, float scale, void* stream) {
   using namespace msc;
-  if (!grad_weights || !logits || !ids || !weights || !grad_logits) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
+  if (tokens != 0 && (!grad_weights || !logits || !ids || !weights || !grad_logits)) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
   if (int rc = check_route(logits, dtype, tokens, experts, topk, score, scale)) return rc;
   if (misaligned(grad_logits, dtype == 1 ? 4 : 2) || misaligned(ids, 4) || misaligned(weights, 4) || misaligned(grad_weights, 4))
     return fail(MSC_ERR_BAD_ARG, "a pointer is not aligned to its type");

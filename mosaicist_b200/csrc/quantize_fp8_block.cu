@@ -340,7 +340,7 @@ extern "C" {
 int msc_fp8_block_quantize(const void* x, int x_dtype, int silu, const int32_t* group_offsets, const int32_t* group_rows,
                            void* q, float* sf, int l, int rows, int k, void* stream) {
   using namespace msc;
-  if (!x || !q || !sf) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
+  if (rows != 0 && (!x || !q || !sf)) return fail(MSC_ERR_BAD_ARG, "NULL pointer");
   if (!group_offsets != !group_rows) return fail(MSC_ERR_BAD_ARG, "group_offsets and group_rows come together");
   if (group_offsets && l <= 0) return fail(MSC_ERR_BAD_ARG, "l=%d must be positive with groups", l);
   if (rows < 0 || k <= 0) return fail(MSC_ERR_BAD_ARG, "rows=%d must not be negative, k=%d must be positive", rows, k);

@@ -533,7 +533,6 @@ std::tuple<Tensor, Tensor> moe_route(const Tensor& logits, int64_t topk, const O
     ids = empty({tokens, topk}, at::kInt, logits);
     weights = empty({tokens, topk}, at::kFloat, logits);
   }
-  if (!tokens) return {*ids, *weights};
   const Lib& f = lib();
   const OnDeviceOf on(logits);
   launch([&] {
@@ -560,7 +559,6 @@ Tensor moe_route_backward(const Tensor& grad, const Tensor& logits, const Tensor
   one_device(logits, {{&ids, "ids"}, {&weights, "weights"}, {&grad, "grad_weights"}, {opt_ptr(out), "out"}});
   const int t = as_int(tokens, "tokens"), e = as_int(experts, "experts"), k = as_int(topk, "topk");
   if (!out) out = empty({tokens, experts}, logits.scalar_type(), logits);
-  if (!tokens) return *out;
   const Lib& f = lib();
   const OnDeviceOf on(logits);
   launch([&] {
@@ -606,7 +604,6 @@ std::tuple<Tensor, Tensor> quantize_fp8_block(const Tensor& x, bool silu, const 
       sf->zero_();
     }
   }
-  if (!total) return {*q, *sf};
   const Lib& f = lib();
   const OnDeviceOf on(x);
   launch([&] {
@@ -673,7 +670,6 @@ Tensor gemm_fp8_block(const Tensor& a_q, const Tensor& a_sf, const Tensor& b_q, 
                    {opt_ptr(row_scale), "row_scale"}, {opt_ptr(out), "out"}});
   const int ll = as_int(l, "l"), tt = as_int(total, "rows"), nn = as_int(n, "n"), kk = as_int(k, "k"), ctas = as_int(max_ctas, "max_ctas");
   if (!out) out = empty({total, n}, kOutTypes[out_type], a_q);
-  if (!total) return *out;
   const Lib& f = lib();
   const OnDeviceOf on(a_q);
   launch([&] {

@@ -257,3 +257,19 @@ def test_fp8_layer_without_a_router_of_its_own(fake, monkeypatch):
     for kw in (dict(), dict(route=None), dict(route=moe.RouteConfig())):
         moe.MegaMoEFp8Block(w1, s1, w2, s2, topk=2, max_tokens=8, **kw).route(_t(8, 4))
     assert seen == [(2, "softmax", None, 1, 1, 1, True, 1.0)] * 3
+
+
+def test_empty_calls_check_their_arguments(lib):
+    """Nothing to do is no reason to take a wrong configuration; what is empty needs no memory."""
+    bad = (_lib.ERR_BAD_ARG, _lib.ERR_UNSUPPORTED)
+    none = dict(logits=None, ids=None, w=None, tokens=0)
+    assert _route(lib, **none) == _lib.OK
+    for cfg in (_cfg(score=2), _cfg(groups=3), _cfg(groups=8, topk_groups=9), _cfg(scale=0.0)):
+        assert _route(lib, cfg=cfg, **none) in bad
+    assert _route(lib, topk=65, **none) in bad
+    back = lambda *a: lib.msc_moe_route_backward(None, None, 1, None, None, None, 0, *a, None)
+    assert back(64, 4, 0, 1, 1.0) == _lib.OK and back(64, 4, 2, 1, 1.0) in bad and back(64, 4, 0, 1, -1.0) in bad and back(64, 0, 0, 1, 1.0) in bad
+    quant = lambda *a: lib.msc_fp8_block_quantize(None, *a, None)
+    assert quant(0, 0, None, None, None, None, 0, 0, 128) == _lib.OK and quant(0, 0, None, None, None, None, 0, 0, 100) in bad
+    gemm = lambda *a: lib.msc_gemm_fp8_block(None, None, P, P, None, *a, None)
+    assert gemm(0, 0, 128, 128, 0) == _lib.OK and gemm(0, 0, 100, 128, 0) in bad and gemm(0, 0, 128, 100, 0) in bad and gemm(5, 0, 128, 128, 0) in bad

@@ -421,3 +421,15 @@ def test_whole_tiles_at_odd_rows(rows):
         out = torch.full((at, n), -3.0, dtype=DT[dtype], device="cuda")
         ops.ragged_grouped_gemm_fp8_block(T(a), _dev_sf(sa), T(b), T(sb), i32(offs), i32(rows), out=out)
         _check(out, want, None, k, dtype, True)
+
+
+def test_empty_batches_check_their_sizes():
+    from mosaicist_b200 import _lib, ops
+
+    u8, f32 = dict(dtype=torch.uint8, device="cuda"), dict(device="cuda")
+    assert ops.quantize_fp8_block(torch.empty(0, 64, **f32))[0].shape == (0, 64)
+    assert ops.gemm_fp8_block(torch.empty(0, 64, **u8), torch.empty(1, 0, **f32), torch.empty(16, 64, **u8), torch.empty(1, 1, **f32)).shape == (0, 16)
+    with pytest.raises(_lib.MscError, match="k=100"):
+        ops.quantize_fp8_block(torch.empty(0, 100, **f32))
+    with pytest.raises(_lib.MscError, match="n=20"):
+        ops.gemm_fp8_block(torch.empty(0, 64, **u8), torch.empty(1, 0, **f32), torch.empty(20, 64, **u8), torch.empty(1, 1, **f32))

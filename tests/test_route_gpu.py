@@ -477,3 +477,15 @@ def test_sigmoids_of_which_some_vanish_in_32_bits(T):
         x[:, e] = rng.integers(lo, hi, T)
     _check(x, 6, score="sigmoid")
     _check(x, 6, score="sigmoid", scale=2.5, bias=np.zeros(64))
+
+
+def test_an_empty_batch_with_a_wrong_configuration():
+    from mosaicist_b200 import _lib, ops
+
+    x, ids, w = torch.empty(0, 64, device="cuda"), torch.empty(0, 4, dtype=torch.int32, device="cuda"), torch.empty(0, 4, device="cuda")
+    assert ops.moe_route(x, 4)[0].shape == (0, 4) and ops.moe_route_backward(w, x, ids, w).shape == (0, 64)
+    for kw in (dict(groups=3), dict(groups=8, topk_groups=9), dict(group_top=3), dict(scale=-1.0)):
+        with pytest.raises(_lib.MscError):
+            ops.moe_route(x, 4, **kw)
+    with pytest.raises(_lib.MscError):
+        ops.moe_route_backward(w, x, ids, w, scale=0.0)
