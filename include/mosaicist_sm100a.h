@@ -317,8 +317,10 @@ int msc_fp8_block_quantize_weight(const void* w, int w_dtype, void* q, float* sf
 
 /* out (m, n) = dequant(a) (m, k) x dequant(b) (n, k)^T, fp32 sums, out_dtype as above.  a_sf as
  * msc_fp8_block_quantize lays it out (pitch = m rounded up to 4), b_sf (ceil(n / 128), ceil(k / 128)).
- * n % 8 == 0; a_q, a_sf, b_q and out are 16-byte aligned.  max_ctas: CTAs of the launch, 0 = all SMs.  m = 0
- * does nothing. */
+ * n % 8 == 0; a_q, a_sf, b_q and out are 16-byte aligned.  max_ctas: CTAs of the launch at most, which come in
+ * pairs (one at least); 0 = all SMs.  A block's two scales are multiplied first, in fp32: where that
+ * product is below 2^-126 bits are lost that the scaled sum would have, where it overflows the sum is
+ * infinite, or NaN if the block's terms add up to 0.  m = 0 does nothing. */
 int msc_gemm_fp8_block(const void* a_q, const float* a_sf, const void* b_q, const float* b_sf, void* out,
                        int out_dtype, int m, int n, int k, int max_ctas, void* stream);
 

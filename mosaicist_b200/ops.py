@@ -303,7 +303,8 @@ def gemm_fp8_block(a_q, a_sf, b_q, b_sf, out_dtype=None, out=None, max_ctas: int
     quantize_fp8_block_weight make them: a_q (m, k), a_sf (ceil(k / 128), m rounded up to 4), b_q (n, k), b_sf
     (ceil(n / 128), ceil(k / 128)); fp32 sums, rounded once to out_dtype (bfloat16 unless `out` or out_dtype
     says float16 or float32).  k % 16 == 0, n % 8 == 0.  Calls of the same sizes give the same bits; a row's last
-    bits may differ from one m to another (small problems are split along k)."""
+    bits may differ from one m to another (small problems are split along k).  max_ctas bounds the launch's CTAs, which come in
+    pairs (0: one on every SM).  The product of a block's two scales is formed in fp32 and has to lie within its normal range."""
     return _host_ops.gemm_fp8_block(a_q, a_sf, b_q, b_sf, _out_type(out_dtype), out, max_ctas)
 
 
