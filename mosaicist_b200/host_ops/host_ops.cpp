@@ -1253,12 +1253,12 @@ TORCH_LIBRARY_IMPL(mosaicist_sm100a, CUDA, m) {
   m.impl("gemm_fp8_block", op_gemm_fp8_block);
   m.impl("grouped_gemm_fp8_block_ragged", op_grouped_gemm_fp8_block_ragged);
 }
-// No operator has a derivative: a backward pass through one raises.  (Without a kernel under this
+// But for moe_route (torch_ops.py) no operator has a derivative: a backward pass through one raises.  (Without a kernel under this
 // key torch only warns and leaves the operator's share out of the gradients.)
 TORCH_LIBRARY_IMPL(mosaicist_sm100a, Autograd, m) {
   for (const char* name : {"grouped_gemm_nvfp4", "grouped_gemm_nvfp4_ragged", "quantize_nvfp4", "silu_mul_quantize_nvfp4",
                            "global_scale_for", "quantize_mxfp8", "grouped_gemm_mxfp8_ragged", "gemm_f16",
-                           "grouped_gemm_bf16_int4_ragged", "moe_masked", "moe_route", "moe_route_backward", "quantize_fp8_block",
+                           "grouped_gemm_bf16_int4_ragged", "moe_masked", "moe_route_backward", "quantize_fp8_block",
                            "quantize_fp8_block_weight", "gemm_fp8_block", "grouped_gemm_fp8_block_ragged"})
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
 }

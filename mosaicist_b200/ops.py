@@ -259,8 +259,15 @@ def moe_route(logits, topk: int, score: str = "softmax", bias=None, groups: int 
     take part.  Ties go to the lower expert (or group), and the order is that of 64-bit arithmetic.
 
     A logit or bias of -inf or NaN bars its expert; where fewer than topk are left, the lowest barred ones
-    fill up, with weight 0.  `out` may carry preallocated (ids, weights).  (The reference has no routing
-    code; MegaMoE's own routing is softmax, no bias, no groups, renormalised.)"""
+    fill up, with weight 0.  `out` may carry preallocated (ids, weights).  Without it the weights of logits
+    that ask for a gradient carry one on (moe_route_backward); into `out` they do not.  (As with any operator of
+    torch, a backward pass is captured into a graph while no eager graph of the same leaves is alive.)  The
+    reference has no routing code; MegaMoE's own routing is softmax, no bias, no groups, renormalised."""
+    if out is None and getattr(logits, "requires_grad", False) and torch.is_grad_enabled():
+        from . import torch_ops
+
+        _score(score)
+        return torch_ops.moe_route(logits, topk, score, bias, groups, topk_groups, group_top, renormalize, scale)
     return _host_ops.moe_route_scores(logits, topk, bias, _score(score), groups, topk_groups, group_top, renormalize, scale,
                                       out)
 

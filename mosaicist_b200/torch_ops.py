@@ -13,7 +13,8 @@ that build graphs of torch operators (tracing, FakeTensor shape propagation) ins
     grouped_gemm_mxfp8_ragged  the MXFP8 grouped GEMM over row-concatenated groups
     gemm_f16                   the dense fp16 / bf16 problem (hopper_gemm/ref_cutedsl.py:50-74)
     grouped_gemm_bf16_int4_ragged   bf16 x int4 grouped GEMM (problems.py:75-87)
-    moe_route, moe_route_backward   expert choices from router logits (ops.moe_route), their gradient
+    moe_route, moe_route_backward   expert choices from router logits (ops.moe_route), their gradient; the first
+                               is differentiable by the second
     quantize_fp8_block[_weight], gemm_fp8_block, grouped_gemm_fp8_block_ragged
                                e4m3 with fp32 scales per block of 128 (ops)
     moe_masked                 the masked MoE layer, arguments of the reference's moe_masked
@@ -157,6 +158,21 @@ def _(logits, topk, score, bias, groups, topk_groups, group_top, renormalize, sc
 @_fake("moe_route_backward")
 def _(grad_weights, logits, ids, weights, score, renormalize, scale):
     return logits.new_empty(logits.shape)
+
+
+def _route_saved(ctx, inputs, output):
+    logits, _, ctx.score, _, _, _, _, ctx.renormalize, ctx.scale = inputs
+    ctx.save_for_backward(logits, *output)
+
+
+def _route_gradient(ctx, _, grad_weights):
+    """By the logits; the choice, and so the bias, has no gradient."""
+    logits, ids, weights = ctx.saved_tensors
+    grad = moe_route_backward(grad_weights.contiguous(), logits, ids, weights, ctx.score, ctx.renormalize, ctx.scale)
+    return grad, None, None, None, None, None, None, None, None
+
+
+torch.library.register_autograd("mosaicist_sm100a::moe_route", _route_gradient, setup_context=_route_saved, lib=_LIBRARY)
 
 
 def _blocks(n):

@@ -489,3 +489,41 @@ def test_an_empty_batch_with_a_wrong_configuration():
             ops.moe_route(x, 4, **kw)
     with pytest.raises(_lib.MscError):
         ops.moe_route_backward(w, x, ids, w, scale=0.0)
+
+
+@pytest.mark.parametrize("score,renormalize,dtype", [("softmax", True, "f32"), ("softmax", False, "bf16"), ("sigmoid", True, "f16"), ("sigmoid", False, "f32")])
+def test_weights_carry_the_gradient_on(score, renormalize, dtype):
+    """ops.moe_route and the torch operator inside a graph of gradients: moe_route_backward's result, also of an expanded
+    gradient; captured and replayed on new data."""
+    import mosaicist_b200.torch_ops as O
+    from mosaicist_b200 import ops
+
+    kw = dict(score=score, groups=4, topk_groups=2, group_top=2, renormalize=renormalize, scale=2.5)
+    bias = torch.randn(64, device="cuda") * 0.1
+    x = torch.randn(300, 64, device="cuda").to(DT[dtype]).requires_grad_()
+    g = torch.randn(300, 6, device="cuda")
+    want_ids, want_w = ops.moe_route(x.detach(), 6, bias=bias, **kw)
+    back = lambda grad, v, ids, w: ops.moe_route_backward(grad, v, ids, w, score, renormalize, 2.5)
+    for ids, w in (ops.moe_route(x, 6, bias=bias, **kw), O.moe_route(x, 6, score, bias, 4, 2, 2, renormalize, 2.5)):
+        assert torch.equal(ids, want_ids) and torch.equal(w, want_w) and w.requires_grad and not ids.requires_grad
+        assert torch.equal(torch.autograd.grad(w, x, g, retain_graph=True)[0], back(g, x.detach(), ids, want_w))
+        assert torch.equal(torch.autograd.grad(w.sum(), x)[0], back(torch.ones_like(g), x.detach(), ids, want_w))
+    with torch.no_grad():
+        assert not ops.moe_route(x, 6, bias=bias, **kw)[1].requires_grad
+    del w, ids
+    leaf = x.detach().clone().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.moe_route(leaf, 6, bias=bias, **kw)[1], leaf, g)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ids, w = ops.moe_route(leaf, 6, bias=bias, **kw)
+        held = torch.autograd.grad(w, leaf, g)[0]
+        w = w.detach()
+    with torch.no_grad():
+        leaf.copy_(x.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(ids, want_ids.flip(0)) and torch.equal(held, back(g, x.detach().flip(0).contiguous(), ids, w))
