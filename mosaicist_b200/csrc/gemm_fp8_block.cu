@@ -22,13 +22,14 @@
 // of K.  And where the last round of a dense product's tiles would keep only a few pairs busy, its tiles are
 // taken in quarters of 64 tokens.
 //
-// What bounds it.  Large products: the consumers.  The MMAs of a K block take 513 cycles, reading 256 columns out of
-// tensor memory, adding them and handing them back about 750, so 8192 x 8192 x 7168 runs in 405 to 417 us, 2.3
-// PFLOP/s, about 70 % of twice the measured bf16 rate (the MX kernel, whose scales the tensor core applies, 307 us).
+// What bounds it.  Large products: the consumers, who read 256 columns of a K block out of tensor memory, add them and hand
+// them back.  The MMAs of a K block take 513 cycles, and a block, with its share of a tile's stores, 890: over 8192 x
+// 8192 x 7168 the tensor pipe is active in 57 % of the cycles, and it runs in 420 to 450 us, 2.1 to 2.3
+// PFLOP/s, 65 to 69 % of twice the measured bf16 rate (the MX kernel, whose scales the tensor core applies, 307 us).
 // Wider or more consumer groups do not fit the registers, scales from a ring in shared memory cost more of its bandwidth
 // than they save (490 us), and accumulators of 128 columns in turn double the hand-overs.  Few tokens: the weights'
-// traffic (64 groups of 0 to 16 rows, 4096 x 7168: 330 us, 5.5 TB/s) or, for one small matrix, the launch
-// and the ring's first fill (16 x 7168 x 2048: 10 us).
+// traffic (64 groups of 0 to 16 rows, 4096 x 7168: 306 us back to back, 338 in turn with others, 5.4 to 6 TB/s) or, for one
+// small matrix, the launch and the ring's first fill (16 x 7168 x 2048: 10 to 12 us).
 #include "gemm_common.cuh"
 #include "quantize_common.cuh"
 

@@ -20,8 +20,10 @@
 // them the serial rounds of choosing.  From 1024 tokens on, and up to 256 experts, eight lanes per token share
 // these rounds among four tokens (below).
 //
-// Neither is bound by memory: 8192 tokens of 256 fp32 logits are 8.9 MB, 1.4 us, and take 12 us with sigmoid,
-// bias and 4 of 8 groups (21 a warp per token), 5 us for 128 bf16 experts without them; 16 tokens take 4 to 5.5 us. What is left
+// Neither is bound by memory: 8192 tokens of 256 fp32 logits are 8.9 MB, 1.4 us, and take 12 to 16 us with sigmoid, bias and
+// 4 of 8 groups, by how many tokens lie close (21 a warp per token), 4.7 us for 128 bf16 experts without them; a warp
+// per token takes 25 us for 8192 x 384 (top 8, sigmoid and bias), 20 for 8192 x 512 (top 10, softmax), 38 for 8192 x 256
+// in 16 groups. 16 tokens take 2.3 to 4 us in a graph, 5.6 launched one by one.  What is left
 // is the chain of one warp's steps (3 to 4 us) and, where keys lie close, the tokens that are looked at in 64 bits.
 //
 // A logit of -inf or NaN, or a bias of -inf or NaN, bars its expert.  Where fewer than topk experts are
@@ -732,9 +734,10 @@ __global__ void __launch_bounds__(32 * kOctetWarps) moe_route_octets_kernel(cons
 //   sigmoid, renormalised   dx_i = w_i (1 - score_i) (g_i - A / scale)
 //   sigmoid                 dx_i = w_i (1 - score_i) g_i
 // A barred expert has weight 0, and so gradient 0.  A warp per token; the row is written whole, then the chosen
-// experts' elements over it.  Bound by the chain of a warp's loads and reductions while tokens are few (1.5 to
-// 2 us), by issue above: 16383 tokens x 160 bf16, softmax as it is, 7.6 us (10.5 MB, 1.6 us of traffic), where
-// rows kept in shared memory took 10.1; 8192 x 256 fp32, chosen experts only, 4.3 us (5.0).  Eight warps a CTA: the same.
+// experts' elements over it.  Bound by the chain of a warp's loads, then of its reductions: 16383 tokens x 160 bf16, softmax as
+// it is, take 7.6 to 7.8 us (10.5 MB, 1.6 us of traffic) with 31 % of the issue slots and 56 % of the warps in use, a
+// warp waiting 9 issues for memory and 5 for shuffles per issue of its own; rows kept in shared memory took 10.1.
+// 8192 x 256 fp32, chosen experts only, 4.4 us (5.0).  Eight warps a CTA: the same.
 struct RouteBackwardParams {
   const void* logits;         // (tokens, experts)
   const int* ids;             // (tokens, topk)
@@ -851,6 +854,7 @@ template <bool SIGMOID, class T>
 static int launch_route_backward(const RouteBackwardParams& p, cudaStream_t stream) {
   cudaLaunchAttribute attr[1];
   cudaLaunchConfig_t lc = pdl_launch_config((p.tokens - 1) / kBackwardWarps + 1, 32 * kBackwardWarps, 0, stream, attr);
+  // (five slots rather than eight: 7.6 us against 7.8 to 7.9 for 72 to 160 experts of 16383 tokens; 8.2 for 192, 10.4 for 384)
   auto kern = SIGMOID || p.renormalize ? moe_route_backward_kernel<0, SIGMOID, T>
               : p.experts <= 64 ? moe_route_backward_kernel<2, false, T>
               : p.experts <= 160 ? moe_route_backward_kernel<5, false, T>

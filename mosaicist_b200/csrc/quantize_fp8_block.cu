@@ -114,9 +114,10 @@ struct RowBlockParams {
 // A CTA takes 8 rows, a warp one of them, and walks its share of the row's pieces of 512 columns with the next
 // piece's loads in flight; a thread holds 16 values, 8 lanes share a block.  The 32 scales of a
 // piece meet in shared memory and leave as 32-byte stretches of the column layout.
-// Measured: gate | up of 16300 rows x 2048 bf16 in 64 groups with silu, 167 MB moved in 36 us, 4.6 TB/s (silu and its
-// two special functions a value keep it below the 5.2 TB/s of 16384 x 7168 without); 16 rows x 7168 in 4.4 us, which is
-// the launch.
+// Measured: gate | up of 16300 rows x 2048 bf16 in 64 groups with silu, 167 MB moved in 36 us, 4.6 TB/s, with half of the issue
+// slots, half of DRAM and 48 % of the special-function pipe in use: 71 registers a thread leave three CTAs on an SM,
+// so that latency is what bounds it.  Without silu (61 registers, four CTAs) 16384 x 7168 takes 68 to 76 us, 4.6 to 5.2
+// TB/s, with 70 to 75 % of the issue slots in use; 16 rows x 7168 4.1 to 4.7 us, which is the launch.
 template <class T, bool SILU>
 __global__ void __launch_bounds__(256) quantize_fp8_rows_kernel(const RowBlockParams p) {
   grid_dependency_wait();
@@ -269,7 +270,8 @@ __global__ void __launch_bounds__(512) moe_permute_quantize_fp8_kernel(const Fp8
 // ---- weights -------------------------------------------------------------------------------
 // A CTA per 128 x 128 block, whose values stay in registers between the maximum and the quotients: a
 // thread holds 64 of them in four row pieces of 16.  Four CTAs an SM keep enough loads in flight: 16 x 4096 x 7168 bf16
-// in 240 us, 5.9 TB/s of read and written bytes, 259 us with two; fp32 values take twice the registers and two CTAs.
+// in 239 us back to back, 5.9 TB/s of read and written bytes, 259 us with two (266 where results go to other memory in every
+// call); fp32 values take twice the registers and two CTAs.
 struct WeightBlockParams {
   const void* w;    // (l, n, k)
   uint8_t* q;       // (l, n, k)
@@ -320,7 +322,7 @@ template <class T>
 static int launch_rows(const RowBlockParams& p, bool silu, cudaStream_t stream) {
   const int sms = num_sms();
   if (sms <= 0) return fail(MSC_ERR_CUDA, "could not query the SM count");
-  // As many CTAs per row as it takes to give every SM sixteen, of which eight are resident: with up to 64 the pieces of
+  // As many CTAs per row as it takes to give every SM sixteen, of which three or four are resident: with up to 64 the pieces of
   // many rows lose their loads in flight (gate | up of 64 groups 52 us against 36), with 4 a middling number
   // of rows fills the SMs badly (4096 x 2048 9.7 us against 8.4).
   const int tiles = (p.rows + 7) / 8, pieces = (p.k + 511) / 512;
