@@ -7,6 +7,7 @@ documented signatures; argument checks, allocation and the launch are native
 
 from __future__ import annotations
 
+import operator
 from dataclasses import dataclass
 
 import torch
@@ -267,7 +268,8 @@ def moe_route(logits, topk: int, score: str = "softmax", bias=None, groups: int 
         from . import torch_ops
 
         _score(score)
-        return torch_ops.moe_route(logits, topk, score, bias, groups, topk_groups, group_top, renormalize, scale)
+        sizes = (operator.index(v) for v in (groups, topk_groups, group_top))
+        return torch_ops.moe_route(logits, operator.index(topk), score, bias, *sizes, bool(renormalize), float(scale))
     return _host_ops.moe_route_scores(logits, topk, bias, _score(score), groups, topk_groups, group_top, renormalize, scale,
                                       out)
 

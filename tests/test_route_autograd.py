@@ -74,6 +74,16 @@ def test_a_step_of_a_router(calls):
     assert float(wr.grad.abs().max()) > 0
 
 
+def test_arguments_as_the_plain_path_takes_them(calls):
+    x = torch.randn(5, 8, requires_grad=True)
+    want = ops.moe_route(x, 2, groups=4, topk_groups=2, renormalize=True, scale=2.0)
+    got = ops.moe_route(x, np.int64(2), groups=np.int32(4), topk_groups=np.int64(2), renormalize=1, scale=2)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for kw in (dict(topk=2.0), dict(topk=2, groups=4.0), dict(topk=2, scale="x")):
+        with pytest.raises((TypeError, ValueError)):
+            ops.moe_route(x, **kw)
+
+
 def test_where_no_gradient_is_asked_for(calls):
     x = torch.randn(5, 8, requires_grad=True)
     with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):      # the plain path, which has no stand-in
